@@ -235,3 +235,87 @@ int mmb_fmha_prefill(const MmbFmhaPrefillParams* p, cudaStream_t stream);
 #ifdef __cplusplus
 }
 #endif
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+// Status word that kernels of this device report to, null where none is registered (bindings.cpp).
+int* mmb_status_word(int device);
+
+// Short causal convolution and selective scan over pools of per-sequence state (causal_conv.cu, ssm_scan.cu).  Element types of the
+// activations: 0 bf16, 1 fp16, 2 fp32; states, A, D and dt_bias are fp32.  rows (int64, may be null: sequence i owns row i) names the
+// pool row of every sequence; a sequence whose row is outside [0, pool_rows) is skipped (outside and not negative: status 130).
+// Prompts: sequence s is the rows cu_seqlens[s] .. cu_seqlens[s + 1] of the activations; fresh[s] != 0 starts it from a zero state; an empty
+// sequence leaves its state alone.  Rows that belong to no live sequence are zeroed in `out` when zero_dead is set, else left alone.
+typedef struct {
+  const void* x;            // [T, C]
+  const void* w;            // [C, K] contiguous
+  const void* bias;         // [C] or null, type of w
+  void* out;                // [T, C]
+  float* state;             // [pool_rows, C, K - 1] contiguous, or null (every sequence fresh, nothing kept)
+  const long long* rows;    // [S] or null
+  const unsigned char* fresh;   // [S] or null; prompts only
+  const int* cu_seqlens;    // [S + 1]; null = single-token step (S = T)
+  long long ldx, ldo;       // row strides in elements
+  int T, S, C, K, pool_rows;
+  int xt, wt, ot;           // element types
+  int act;                  // 0 none, 1 SiLU
+  int zero_dead;
+  int* status;
+} MmbCausalConvParams;
+int mmb_causal_conv(const MmbCausalConvParams* p, cudaStream_t stream);
+int mmb_causal_conv_step(const MmbCausalConvParams* p, cudaStream_t stream);
+
+typedef struct {
+  const void* x;            // [T, D]
+  const void* dt;           // [T, D]
+  const void* z;            // [T, D] or null
+  const void* B;            // [T, N]
+  const void* C;            // [T, N], type of B
+  const float* A;           // [D, N] contiguous
+  const float* Dskip;       // [D] or null
+  const float* dt_bias;     // [D] or null
+  void* out;                // [T, D]
+  float* state;             // [pool_rows, D, N] contiguous, or null (prompts only)
+  const long long* rows;
+  const unsigned char* fresh;
+  const int* cu_seqlens;    // null = single-token step
+  long long ldx, lddt, ldz, ldb, ldc, ldo;
+  int T, S, D, N, pool_rows;
+  int xt, dtt, zt, bt, ot;
+  int softplus;
+  int zero_dead;
+  int* status;
+} MmbSsmParams;
+int mmb_ssm_scan(const MmbSsmParams* p, cudaStream_t stream);
+int mmb_ssm_step(const MmbSsmParams* p, cudaStream_t stream);
+#ifdef __cplusplus
+}
+#endif
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+// Attention of one new token per sequence over a paged pool, visible keys p < sinks or p >= ctx - window (attention_sinks.cu).  K / V pools
+// [n_slots, Hkv, D] bf16 (fmt -1) or codes with fp32 row scales [n_slots, Hkv] (fmt 0 E4M3, 1 int8, 2 E2M1, 3 int4; the 4-bit formats hold
+// the even element in the low nibble).  D is 64, 128 or 256.  A block table entry outside the pool hides its tokens and reports status 131.
+typedef struct {
+  const void* q;            // bf16 [B, Hq, D] contiguous
+  const void* k;
+  const void* v;
+  const float* k_scale;
+  const float* v_scale;
+  const int* block_tables;  // [B, max_blocks]
+  const int* ctx_lens;      // [B]
+  void* out;                // bf16 [B, Hq, D] contiguous
+  int B, Hq, Hkv, D, block_size, max_blocks, fmt;
+  long long n_slots;
+  int window, sinks;        // window >= 1
+  float scale;
+  int splits;               // CTAs that share a (sequence, KV head): 1, 2, 4, 8; 0 = the launcher's choice
+  int* status;
+} MmbSinkDecodeParams;
+int mmb_sink_decode(const MmbSinkDecodeParams* p, cudaStream_t stream);
+#ifdef __cplusplus
+}
+#endif

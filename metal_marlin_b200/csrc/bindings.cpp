@@ -938,6 +938,8 @@ void bf16_gemm_impl(const Tensor& x, const Tensor& w, Tensor out, Tensor status,
 
 }  // namespace
 
+int* mmb_status_word(int device) { return (device >= 0 && device < 64) ? g_status_word[device] : nullptr; }
+
 // ------------------------------------------------------------------------------------------------ secondary kernels
 void hadamard(const Tensor& x, Tensor out, int64_t block) {
   check_bf16(x, "x");

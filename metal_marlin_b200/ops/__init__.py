@@ -507,10 +507,21 @@ def default_splits(batch: int, n_kv_heads: int, max_ctx: int, sm_count: int = 14
 
 
 def paged_attention(q, k_pool, v_pool, block_tables, ctx_lens, *, Hq, Hkv, dqk, dv, block_size, scale, window=0,
-                    splits=None, w_uv=None, workspace=None, out=None, max_ctx=None):
+                    splits=None, w_uv=None, workspace=None, out=None, max_ctx=None, sinks=0):
     """Decode attention over a paged pool.  With ``w_uv [Hq, dvo, dv]`` the merged latent output is
-    up-projected per head (MLA).  Returns bf16 ``[B, Hq, dvo or dv]``."""
+    up-projected per head (MLA).  Returns bf16 ``[B, Hq, dvo or dv]``.
+
+    ``window > 0``: the new token sees the last ``window`` tokens of its sequence, itself included; with ``sinks > 0`` the first
+    ``sinks`` tokens stay visible too (the mask of :func:`prefill_attention`).  Sinks take per-head K / V pools of any cache
+    format and head sizes 64, 128 and 256; one launch splits and joins by itself (``csrc/attention_sinks.cu``), so ``splits`` and
+    ``workspace`` do not apply.  A sequence without tokens gives zeros; a block outside the pool hides its tokens and is
+    reported by :func:`check_status`."""
     B = ctx_lens.numel()
+    if sinks:
+        if sinks < 0 or window < 0:
+            raise ValueError(f"window and sinks must not be negative, got {window} and {sinks}")
+        if window > 0:
+            return _sink_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv, block_size, scale, window, sinks, w_uv, out)
     dvo = w_uv.shape[1] if w_uv is not None else dv
     fp8 = isinstance(k_pool, FP8KV)
     if not _use_native(q):
@@ -543,6 +554,128 @@ def paged_attention(q, k_pool, v_pool, block_tables, ctx_lens, *, Hq, Hkv, dqk, 
         K.mmb200.paged_decode(q, k_pool, v_pool, block_tables, ctx_lens, part_o, part_ml, Hq, Hkv, dqk, dv, block_size,
                               splits, scale, window)
     K.mmb200.decode_merge(part_o, part_ml, w_uv, out, B, Hq, dv, dvo, splits)
+    return out
+
+
+def _sink_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv, block_size, scale, window, sinks, w_uv, out):
+    if v_pool is None or w_uv is not None or dqk != dv:
+        raise ValueError("attention with sinks takes K and V pools of one head size (no latent cache)")
+    quant = isinstance(k_pool, FP8KV)
+    if quant and not (isinstance(v_pool, FP8KV) and v_pool.fmt == k_pool.fmt):
+        raise ValueError("K and V pools must have one cache format")
+    B = ctx_lens.numel()
+    if not _use_native(q):
+        if dv not in PREFILL_ATTN_DIMS:
+            raise ValueError(f"attention with sinks takes head sizes 64, 128 and 256, got {dv}")
+        if Hkv < 1 or Hq % Hkv:
+            raise ValueError("query heads must be a multiple of KV heads")
+        if quant:
+            k_pool, v_pool = k_pool.dequantize(), v_pool.dequantize()
+        o = ref.paged_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv, block_size, scale, window, sinks)
+        if out is not None:
+            out.copy_(o.view_as(out))
+            return out
+        return o
+    if out is None:
+        out = torch.empty(B, Hq, dv, dtype=torch.bfloat16, device=q.device)
+    _report_on(q.device)
+    if quant:
+        K.mmb200.sink_decode(q.contiguous(), k_pool.data, v_pool.data, k_pool.scale, v_pool.scale, block_tables, ctx_lens, out, Hq, Hkv, dv, block_size,
+                             scale, window, sinks, k_pool.fmt_code, 0)
+    else:
+        K.mmb200.sink_decode(q.contiguous(), k_pool, v_pool, None, None, block_tables, ctx_lens, out, Hq, Hkv, dv, block_size, scale, window, sinks, -1, 0)
+    return out
+
+
+_reporting = set()
+
+
+def _report_on(device) -> None:
+    """Registers the device's status word on first use (kernels report bad block tables and pool rows there)."""
+    if device not in _reporting:
+        gemm_status(device)
+        _reporting.add(device)
+
+
+def _stream_out(x, out, out_dtype, *inputs):
+    """The output of a call over token rows: a new tensor, or the caller's after a check that no input of other rows lies in it."""
+    if out is None:
+        return torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+    if out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
+    for t in inputs:
+        if t is None or t.numel() == 0 or out.numel() == 0 or t.untyped_storage().data_ptr() != out.untyped_storage().data_ptr():
+            continue
+        lo, hi, e = out.data_ptr(), t.data_ptr(), t.element_size()
+        if lo < hi + ((t.shape[0] - 1) * t.stride(0) + t.shape[-1]) * e and hi < lo + ((out.shape[0] - 1) * out.stride(0) + out.shape[-1]) * out.element_size():
+            # side by side in the rows of one wider buffer is fine
+            pitch = t.stride(0) * e
+            gap = (lo - hi) % pitch if pitch else 0
+            if out.stride(0) * out.element_size() != pitch or gap < t.shape[-1] * e or gap + out.shape[-1] * out.element_size() > pitch:
+                raise ValueError("out must not overlap an input")
+    return out
+
+
+def causal_conv(x, w, bias=None, *, cu_seqlens, state=None, rows=None, fresh=None, act=1, out=None, out_dtype=None):
+    """Short causal depthwise convolution of a ragged batch of prompts, the one in front of Mamba and Gated DeltaNet mixers:
+    ``y[t, c] = silu(bias[c] + sum_k w[c, k] x[t - K + 1 + k, c])`` (``act=0``: no SiLU).
+
+    ``x [T, C]`` (bf16, fp16 or fp32, any row stride), ``w [C, K]`` with ``K`` 2 to 8, ``bias [C]`` of ``w``'s type.  Sequence ``i`` is the rows
+    ``cu_seqlens[i] .. cu_seqlens[i + 1]`` (int32 ``[S + 1]`` on the device, starting at 0).  ``state`` fp32 ``[P, C, K - 1]`` is a pool of
+    windows, the last inputs of each sequence with the oldest first: sequence ``i`` continues from row ``rows[i]`` (int64; row ``i``
+    without ``rows``), or from zeros where ``fresh[i]`` is set, and leaves its new window there.  Without a pool every sequence starts
+    from zeros.  A sequence with a negative row is skipped, an empty one leaves its window alone; rows of ``x`` that belong to no
+    sequence give zeros (in a caller's ``out``: are left as they were).  Live sequences must have different rows.
+    Kernel: ``csrc/causal_conv.cu``; single tokens: :func:`causal_conv_step`."""
+    zero = out is None
+    out = _stream_out(x, out, out_dtype, x)
+    if not _use_native(x):
+        return ref.causal_conv(x, w, bias, cu_seqlens, state, rows, fresh, act, out, zero)
+    _report_on(x.device)
+    K.mmb200.causal_conv(x, w, bias, out, state, rows, fresh, cu_seqlens, act, zero)
+    return out
+
+
+def causal_conv_step(x, w, bias=None, *, state, rows=None, act=1, out=None, out_dtype=None):
+    """One new token per sequence of :func:`causal_conv`: ``x [B, C]``, row ``i`` continues from ``state[rows[i]]`` (row ``i`` without
+    ``rows``) and shifts that window by its input.  A negative row is a padding row: its output is zero (in a caller's ``out``: left
+    as it was)."""
+    zero = out is None
+    out = _stream_out(x, out, out_dtype, x)
+    if not _use_native(x):
+        return ref.causal_conv(x, w, bias, None, state, rows, None, act, out, zero)
+    _report_on(x.device)
+    K.mmb200.causal_conv(x, w, bias, out, state, rows, None, None, act, zero)
+    return out
+
+
+def ssm_scan(x, dt, A, Bm, Cm, *, cu_seqlens, state=None, rows=None, fresh=None, D=None, z=None, dt_bias=None, dt_softplus=False, out=None,
+             out_dtype=None):
+    """Selective state space scan of a ragged batch of prompts (Mamba): with ``d = softplus(dt + dt_bias)`` (``dt_softplus=False``: no
+    softplus), ``h <- exp(d A) h + d x B_t``, ``y_t = <h, C_t> + D x_t``, ``out = y silu(z)``.
+
+    ``x, dt, z [T, Di]`` and ``Bm, Cm [T, N]`` are bf16, fp16 or fp32 (``Bm`` and ``Cm`` alike) with any row stride, so they can be slices of a
+    projection's output; ``A [Di, N]`` (negative), ``D`` and ``dt_bias [Di]`` fp32, ``N`` 1 to 128.  ``state`` fp32 ``[P, Di, N]`` is a pool of
+    states that is read where a sequence starts and written where it ends; ``cu_seqlens``, ``rows``, ``fresh``, skipped and empty
+    sequences and rows behind the last one as in :func:`causal_conv`.  Kernel: ``csrc/ssm_scan.cu``; single tokens: :func:`ssm_step`."""
+    zero = out is None
+    out = _stream_out(x, out, out_dtype, x, dt, z, Bm, Cm)
+    if not _use_native(x):
+        return ref.ssm(x, dt, A, Bm, Cm, D, z, dt_bias, cu_seqlens, state, rows, fresh, dt_softplus, out, zero)
+    _report_on(x.device)
+    K.mmb200.ssm(x, dt, A, Bm, Cm, D, z, dt_bias, out, state, rows, fresh, cu_seqlens, dt_softplus, zero)
+    return out
+
+
+def ssm_step(x, dt, A, Bm, Cm, *, state, rows=None, D=None, z=None, dt_bias=None, dt_softplus=False, out=None, out_dtype=None):
+    """One new token per sequence of :func:`ssm_scan`: ``x, dt, z [B, Di]``, ``Bm, Cm [B, N]``; row ``i`` updates ``state[rows[i]]`` in place (row
+    ``i`` without ``rows``).  A negative row is a padding row: its output is zero (in a caller's ``out``: left as it was)."""
+    zero = out is None
+    out = _stream_out(x, out, out_dtype, x, dt, z, Bm, Cm)
+    if not _use_native(x):
+        return ref.ssm(x, dt, A, Bm, Cm, D, z, dt_bias, None, state, rows, None, dt_softplus, out, zero)
+    _report_on(x.device)
+    K.mmb200.ssm(x, dt, A, Bm, Cm, D, z, dt_bias, out, state, rows, None, None, dt_softplus, zero)
     return out
 
 

@@ -170,8 +170,9 @@ def mla_prep(q, kva, w_ukT, kv_norm_w, positions, inv_freq, slots, q_full, cache
     return q_full
 
 
-def paged_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv, block_size, scale, window=0):
-    """Returns bf16 [B, Hq, dv].  ``v_pool`` None means V = K[..., :dv] (MLA latent)."""
+def paged_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv, block_size, scale, window=0, sinks=0):
+    """Returns bf16 [B, Hq, dv].  ``v_pool`` None means V = K[..., :dv] (MLA latent).  With a window the first ``sinks`` keys
+    stay visible."""
     B = ctx_lens.numel()
     out = torch.zeros(B, Hq, dv, dtype=torch.float32, device=q.device)
     Gh = Hq // Hkv
@@ -183,6 +184,8 @@ def paged_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv,
             continue
         lo = max(0, n - window) if window > 0 else 0
         tok = torch.arange(lo, n, device=q.device)
+        if sinks and lo:
+            tok = torch.cat([torch.arange(min(sinks, lo), device=q.device), tok])
         slots = block_tables[b, tok // block_size].long() * block_size + (tok % block_size)
         K = kp[slots].to(torch.float32)                                   # [n, Hkv, dqk]
         V = vp[slots].to(torch.float32) if vp is not None else K[..., :dv]
@@ -191,6 +194,130 @@ def paged_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv,
         p = torch.softmax(s, dim=-1)
         out[b] = torch.einsum("hgn,nhd->hgd", p, V).reshape(Hq, dv)
     return out.to(torch.bfloat16)
+
+
+def _need(ok, message: str) -> None:
+    if not ok:
+        raise ValueError(message)
+
+
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _check_2d(t, rows, cols, on, name) -> None:
+    _need(t.dim() == 2 and t.shape[0] == rows and t.shape[1] == cols, f"{name} must have the shape [{rows}, {cols}]")
+    _need(t.stride(1) == 1 or cols <= 1, f"{name} must have unit stride along its last axis")
+    _need(t.device == on.device, f"{name} must be on the device of x")
+    _need(t.dtype in _FLOATS, f"{name} must be bf16, fp16 or fp32")
+
+
+def _sequences(x, state, c, n, rows, fresh, cu):
+    """Checks of a call over pooled per-sequence state (those of the CUDA binding), then ``(first row, length, pool row or None, starts
+    anew)`` of every sequence that is neither empty nor skipped."""
+    S = x.shape[0]
+    if cu is not None:
+        _need(cu.dtype == torch.int32 and cu.dim() == 1 and cu.numel() >= 1 and cu.is_contiguous() and cu.device == x.device,
+              "cu_seqlens must be a contiguous int32 vector on the device of x")
+        S = cu.numel() - 1
+    if state is not None:
+        _need(state.dtype == torch.float32 and state.is_contiguous() and state.dim() == 3 and tuple(state.shape[1:]) == (c, n),
+              f"state must be a contiguous fp32 pool [rows, {c}, {n}]")
+        _need(state.device == x.device, "state must be on the device of x")
+    else:
+        _need(cu is not None, "a single-token step needs a state pool")
+        _need(rows is None, "rows name places of a state pool: pass state too")
+    if rows is not None:
+        _need(rows.dtype == torch.int64 and rows.dim() == 1 and rows.numel() == S and rows.is_contiguous() and rows.device == x.device,
+              f"rows must be a contiguous int64 vector with one entry per sequence ({S}) on the device of x")
+    elif state is not None:
+        _need(state.shape[0] >= S, f"without rows, sequence i owns row i of state: it needs {S} rows")
+    if fresh is not None:
+        _need(fresh.dtype in (torch.bool, torch.uint8) and fresh.dim() == 1 and fresh.numel() == S and fresh.is_contiguous() and fresh.device == x.device,
+              f"fresh must be a contiguous bool or uint8 vector with one entry per sequence ({S}) on the device of x")
+    at = [0] * (S + 1) if S == 0 else (cu.tolist() if cu is not None else list(range(S + 1)))
+    own = rows.tolist() if rows is not None else list(range(S))
+    new = fresh.tolist() if fresh is not None else [False] * S
+    out = []
+    for i in range(S):
+        b = min(max(at[i], 0), x.shape[0])
+        length = min(max(at[i + 1], b), x.shape[0]) - b
+        if length > 0 and (state is None or 0 <= own[i] < state.shape[0]):
+            out.append((b, length, None if state is None else own[i], bool(new[i])))
+    return out
+
+
+def causal_conv(x, w, bias, cu_seqlens, state, rows, fresh, act, out, zero_dead):
+    """Short causal depthwise convolution (``cu_seqlens`` None: one token per row)."""
+    _need(x.dim() == 2, "x must be [tokens, channels]")
+    T, C = x.shape
+    _check_2d(x, T, C, x, "x")
+    _need(w.dim() == 2 and w.shape[0] == C and 2 <= w.shape[1] <= 8 and w.is_contiguous(), f"w must be contiguous [{C}, 2 .. 8]")
+    _need(w.device == x.device, "w must be on the device of x")
+    _need(w.dtype in _FLOATS, "w must be bf16, fp16 or fp32")
+    _check_2d(out, T, C, x, "out")
+    _need(act in (0, 1), "act must be 0 (none) or 1 (SiLU)")
+    if bias is not None:
+        _need(bias.numel() == C and bias.is_contiguous() and bias.dtype == w.dtype and bias.device == x.device,
+              f"bias must hold {C} values of w's type on the device of x")
+    K = w.shape[1]
+    live = _sequences(x, state, C, K - 1, rows, fresh, cu_seqlens)
+    xf, wf = x.float(), w.float()
+    if zero_dead:
+        out.zero_()
+    for b, n, row, new in live:
+        win = torch.zeros(C, K - 1, device=x.device) if row is None or new else state[row]
+        line = torch.cat([win, xf[b: b + n].t()], 1)                          # [C, K - 1 + n]
+        y = sum(line[:, k: k + n] * wf[:, k: k + 1] for k in range(K))
+        if bias is not None:
+            y = y + bias.float()[:, None]
+        if act == 1:
+            y = y * torch.sigmoid(y)
+        out[b: b + n] = y.t().to(out.dtype)
+        if row is not None:
+            state[row] = line[:, n:]
+    return out
+
+
+def ssm(x, dt, A, Bm, Cm, D, z, dt_bias, cu_seqlens, state, rows, fresh, softplus, out, zero_dead):
+    """Selective state space scan (``cu_seqlens`` None: one token per row)."""
+    _need(x.dim() == 2, "x must be [tokens, channels]")
+    T, Di = x.shape
+    _check_2d(x, T, Di, x, "x")
+    _check_2d(dt, T, Di, x, "dt")
+    _need(A.dim() == 2 and A.shape[0] == Di and 1 <= A.shape[1] <= 128 and A.dtype == torch.float32 and A.is_contiguous() and A.device == x.device,
+          f"A must be contiguous fp32 [{Di}, 1 .. 128] on the device of x")
+    N = A.shape[1]
+    _check_2d(Bm, T, N, x, "Bm")
+    _check_2d(Cm, T, N, x, "Cm")
+    _need(Bm.dtype == Cm.dtype, "Bm and Cm must have one type")
+    _check_2d(out, T, Di, x, "out")
+    if z is not None:
+        _check_2d(z, T, Di, x, "z")
+    for t, name in ((D, "D"), (dt_bias, "dt_bias")):
+        if t is not None:
+            _need(t.dtype == torch.float32 and t.is_contiguous() and t.numel() == Di, f"{name} must be contiguous fp32 of {Di} values")
+            _need(t.device == x.device, f"{name} must be on the device of the activations")
+    live = _sequences(x, state, Di, N, rows, fresh, cu_seqlens)
+    xf, Bf, Cf = x.float(), Bm.float(), Cm.float()
+    d = dt.float() if dt_bias is None else dt.float() + dt_bias
+    if softplus:
+        d = d.clamp(min=0) + torch.log1p(torch.exp(-d.abs()))
+    if zero_dead:
+        out.zero_()
+    for b, n, row, new in live:
+        h = torch.zeros(Di, N, device=x.device) if row is None or new else state[row].clone()
+        for t in range(b, b + n):
+            h = torch.exp(d[t, :, None] * A) * h + (d[t] * xf[t])[:, None] * Bf[t]
+            y = (h * Cf[t]).sum(-1)
+            if D is not None:
+                y = y + D * xf[t]
+            if z is not None:
+                zf = z[t].float()
+                y = y * zf * torch.sigmoid(zf)
+            out[t] = y.to(out.dtype)
+        if row is not None:
+            state[row] = h
+    return out
 
 
 def mla_up(o_lat, w_uv):
