@@ -3,7 +3,7 @@
 // where inputs in front of a sequence come from its window state[row, c, 0 .. K - 2] (oldest first), which afterwards holds the sequence's
 // last K - 1 inputs.  2 K flops against one value read and one written: bound by memory at every size that fills the GPU.
 //
-// Prompts.  A thread owns V neighbouring channels (16 bytes of a 16-bit type) and walks TT tokens of one sequence with the last K - 1
+// Prompts.  A thread owns V = 4 neighbouring channels (one where the rows are not aligned for that) and walks TT tokens of one sequence with the last K - 1
 // inputs in registers, so an input is read (TT + K - 1) / TT times, the repeats from L2.  Tiles are cut per sequence, not over the flat
 // token axis: with TT >= K - 1 only a sequence's first tile reads its old window, and the same thread writes the new one (from x, or from
 // the old window where the sequence is shorter than it), so the window can be updated in place without a second launch.  Tile i belongs to
@@ -22,9 +22,35 @@ constexpr int kConvThreads = 128;
 
 __device__ __forceinline__ float conv_act(float y, int act) { return act == 1 ? silu(y) : y; }
 
-template <int K, int V>
+// Taps and bias of V channels; taps that are compiled in but not used are zero.  The V K values of 16-bit weights lie together: whole words.
+template <int KT, int V>
+__device__ __forceinline__ void load_taps(const MmbCausalConvParams& p, int c0, int K, float (&w)[KT][V], float (&b)[V]) {
+  const int skip = KT - K;
+  const long long at = (long long)c0 * K;
+  if (KT < 8 && KT * V % 8 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0) {
+    float f[KT * V];
+#pragma unroll
+    for (int i = 0; i < KT * V / 8; ++i) ldv<8>(p.w, at + 8 * i, p.wt, f + 8 * i);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int k = 0; k < KT; ++k) w[k][v] = f[v * KT + k];
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int k = 0; k < KT; ++k) w[k][v] = k >= skip ? ld1(p.w, at + v * K + k - skip, p.wt) : 0.f;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) b[v] = p.bias ? ld1(p.bias, c0 + v, p.wt) : 0.f;
+}
+
+// KT taps are compiled in; `K` of them are used (K < KT only for KT = 8), aligned to the newest input: tap KT - 1 meets the newest one.
+template <int KT, int V, int ES>
 __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCausalConvParams p, int n_groups, int TT, long long n_tiles) {
-  constexpr int U = V == 8 ? 4 : 8;        // tokens loaded together
+  constexpr int U = V == 4 && ES == 4 ? 4 : 8;             // tokens loaded together
+  constexpr int W = KT - 1;
+  const int K = KT == 8 ? p.K : KT, skip = KT - K;
   pdl_launch_dependents();
   pdl_wait();
   const long long id = (long long)blockIdx.x * kConvThreads + threadIdx.x;
@@ -36,11 +62,11 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCaus
   int lo = 0, hi = p.S;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if ((long long)start(mid) / TT + mid <= tile) lo = mid;
+    if (start(mid) / TT + mid <= tile) lo = mid;
     else hi = mid - 1;
   }
   const int s = lo, begin = start(s), end = s < p.S ? max(begin, start(s + 1)) : p.T;
-  const long long first = (tile - ((long long)begin / TT + s)) * TT;
+  const long long first = (tile - (begin / TT + s)) * TT;
   if (first < 0 || first >= end - begin) return;
   const int t0 = begin + (int)first, t1 = min(end, t0 + TT);
   long long row = -1;
@@ -56,36 +82,40 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCaus
     }
     return;
   }
-  float w[K][V], b[V], win[K - 1][V];
+  Raw<V, ES> xr[U];
+  auto load = [&](int t) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
+    for (int u = 0; u < U; ++u)
+      if (t + u < t1) ld_raw<V, ES>(p.x, (long long)(t + u) * p.ldx + c0, xr[u]);
+  };
+  load(t0);
+  float w[KT][V], b[V], win[W][V];
+  Raw<V, ES> wr[W];
+  if (first > 0) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) w[k][v] = ld1(p.w, (long long)(c0 + v) * K + k, p.wt);
-    b[v] = p.bias ? ld1(p.bias, c0 + v, p.wt) : 0.f;
+    for (int j = 0; j < W; ++j)
+      if (j >= skip) ld_raw<V, ES>(p.x, (long long)(t0 - W + j) * p.ldx + c0, wr[j]);
   }
+  load_taps<KT, V>(p, c0, K, w, b);
   if (first == 0) {
     const bool old = p.state && !(p.fresh && p.fresh[s]);
-    float* st = p.state ? p.state + (row * p.C + c0) * (K - 1) : nullptr;
+    float* st = p.state ? p.state + (row * p.C + c0) * (K - 1) - skip : nullptr;
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
-      for (int j = 0; j < K - 1; ++j) win[j][v] = old ? st[v * (K - 1) + j] : 0.f;
+      for (int j = 0; j < W; ++j) win[j][v] = old && j >= skip ? st[v * (K - 1) + j] : 0.f;
     if (st) {
       const int len = end - begin;
 #pragma unroll
-      for (int j = 0; j < K - 1; ++j) {
-        const int at = len - (K - 1) + j;        // place of the new window's element j in the sequence
+      for (int j = 0; j < W; ++j) {
+        if (j < skip) continue;
+        const int at = len - W + j;              // place of the new window's element j in the sequence; before it, in the old window
         float nw[V];
         if (at >= 0) {
           ldv<V>(p.x, (long long)(begin + at) * p.ldx + c0, p.xt, nw);
         } else {
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            nw[v] = 0.f;
-#pragma unroll
-            for (int i = 0; i < K - 1; ++i)
-              if (i == j + len) nw[v] = win[i][v];
-          }
+          for (int v = 0; v < V; ++v) nw[v] = old ? st[v * (K - 1) + j + len] : 0.f;      // behind what has been overwritten
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) st[v * (K - 1) + j] = nw[v];
@@ -93,71 +123,75 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCaus
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) ldv<V>(p.x, (long long)(t0 - (K - 1) + j) * p.ldx + c0, p.xt, win[j]);
+    for (int j = 0; j < W; ++j) {
+      if (j >= skip) {
+        cvt_raw<V, ES>(wr[j], p.xt, win[j]);
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) win[j][v] = 0.f;
+      }
+    }
   }
   for (int t = t0; t < t1; t += U) {
-    float x[U][V];
+    Raw<V, ES> now[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (t + u < t1) ldv<V>(p.x, (long long)(t + u) * p.ldx + c0, p.xt, x[u]);
+    for (int u = 0; u < U; ++u) now[u] = xr[u];
+    if (t + U < t1) load(t + U);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (t + u < t1) {
-        float y[V];
+      float x[V], y[V];
+      cvt_raw<V, ES>(now[u], p.xt, x);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          float a = b[v];
+      for (int v = 0; v < V; ++v) {
+        float a = b[v];
 #pragma unroll
-          for (int k = 0; k < K - 1; ++k) a = fmaf(w[k][v], win[k][v], a);
-          y[v] = conv_act(fmaf(w[K - 1][v], x[u][v], a), p.act);
-        }
-        stv<V>(p.out, (long long)(t + u) * p.ldo + c0, p.ot, y);
+        for (int k = 0; k < W; ++k) a = fmaf(w[k][v], win[k][v], a);
+        y[v] = conv_act(fmaf(w[W][v], x[v], a), p.act);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-#pragma unroll
-          for (int k = 0; k + 1 < K - 1; ++k) win[k][v] = win[k + 1][v];
-          win[K - 2][v] = x[u][v];
-        }
+        for (int k = 0; k + 1 < W; ++k) win[k][v] = win[k + 1][v];
+        win[W - 1][v] = x[v];
       }
+      if (t + u < t1) stv<V>(p.out, (long long)(t + u) * p.ldo + c0, p.ot, y);
     }
   }
 }
 
-template <int K, int V, int RB>
+template <int KT, int V, int ES, int RB>
 __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(const MmbCausalConvParams p, int n_groups) {
+  constexpr int W = KT - 1;
+  const int K = KT == 8 ? p.K : KT, skip = KT - K;
+  constexpr bool kVecState = V == 4 && KT < 8;
   pdl_launch_dependents();
   pdl_wait();
   const int g = blockIdx.x * kConvThreads + threadIdx.x;
   if (g >= n_groups) return;
   const int c0 = g * V;
-  float w[K][V], b[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) w[k][v] = ld1(p.w, (long long)(c0 + v) * K + k, p.wt);
-    b[v] = p.bias ? ld1(p.bias, c0 + v, p.wt) : 0.f;
-  }
   const int r0 = blockIdx.y * RB;
-  float win[RB][V * (K - 1)], x[RB][V];
   long long row[RB];
+  float win[RB][V * W];
+  Raw<V, ES> xr[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) row[r] = r0 + r < p.T ? pool_row(p.rows, r0 + r, p.pool_rows, p.status) : -1;
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
-    row[r] = r0 + r < p.T ? pool_row(p.rows, r0 + r, p.pool_rows, p.status) : -1;
-    if (row[r] >= 0) {
-      const float* st = p.state + (row[r] * p.C + c0) * (K - 1);
-      if constexpr (V == 4) {
+    if (row[r] < 0) continue;
+    const float* st = p.state + (row[r] * p.C + c0) * (K - 1);
+    if constexpr (kVecState) {
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) {
-          const float4 f = reinterpret_cast<const float4*>(st)[j];
-          win[r][4 * j] = f.x, win[r][4 * j + 1] = f.y, win[r][4 * j + 2] = f.z, win[r][4 * j + 3] = f.w;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < V * (K - 1); ++j) win[r][j] = st[j];
+      for (int j = 0; j < W; ++j) {
+        const float4 f = reinterpret_cast<const float4*>(st)[j];
+        win[r][4 * j] = f.x, win[r][4 * j + 1] = f.y, win[r][4 * j + 2] = f.z, win[r][4 * j + 3] = f.w;
       }
-      ldv<V>(p.x, (long long)(r0 + r) * p.ldx + c0, p.xt, x[r]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int j = 0; j < W; ++j) win[r][v * W + j] = j >= skip ? st[v * (K - 1) + j - skip] : 0.f;
     }
+    ld_raw<V, ES>(p.x, (long long)(r0 + r) * p.ldx + c0, xr[r]);
   }
+  float w[KT][V], b[V];
+  load_taps<KT, V>(p, c0, K, w, b);
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
     if (row[r] < 0) {
@@ -167,56 +201,66 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(const Mm
       }
       continue;
     }
-    float y[V], nw[V * (K - 1)];
+    float x[V], y[V], nw[V * W];
+    cvt_raw<V, ES>(xr[r], p.xt, x);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float a = b[v];
 #pragma unroll
-      for (int k = 0; k < K - 1; ++k) {
-        a = fmaf(w[k][v], win[r][v * (K - 1) + k], a);
-        nw[v * (K - 1) + k] = k + 1 < K - 1 ? win[r][v * (K - 1) + k + 1] : x[r][v];
+      for (int k = 0; k < W; ++k) {
+        a = fmaf(w[k][v], win[r][v * W + k], a);
+        nw[v * W + k] = k + 1 < W ? win[r][v * W + k + 1] : x[v];
       }
-      y[v] = conv_act(fmaf(w[K - 1][v], x[r][v], a), p.act);
+      y[v] = conv_act(fmaf(w[W][v], x[v], a), p.act);
     }
     float* st = p.state + (row[r] * p.C + c0) * (K - 1);
-    if constexpr (V == 4) {
+    if constexpr (kVecState) {
 #pragma unroll
-      for (int j = 0; j < K - 1; ++j) reinterpret_cast<float4*>(st)[j] = make_float4(nw[4 * j], nw[4 * j + 1], nw[4 * j + 2], nw[4 * j + 3]);
+      for (int j = 0; j < W; ++j) reinterpret_cast<float4*>(st)[j] = make_float4(nw[4 * j], nw[4 * j + 1], nw[4 * j + 2], nw[4 * j + 3]);
     } else {
 #pragma unroll
-      for (int j = 0; j < V * (K - 1); ++j) st[j] = nw[j];
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+          if (j >= skip) st[v * (K - 1) + j - skip] = nw[v * W + j];
     }
     stv<V>(p.out, (long long)(r0 + r) * p.ldo + c0, p.ot, y);
   }
 }
 
-template <int K>
-static int launch_conv(const MmbCausalConvParams& p, cudaStream_t stream) {
-  const bool vec = p.C % 8 == 0 && rows_aligned(p.x, p.ldx, p.xt, 8) && rows_aligned(p.out, p.ldo, p.ot, 8);
-  const int groups = vec ? p.C / 8 : p.C;
-  const int TT = (long long)p.T * groups >= (1 << 21) ? 32 : 8;
+template <int KT, int V, int ES>
+static int launch_conv_v(const MmbCausalConvParams& p, cudaStream_t stream) {
+  const int groups = p.C / V;
+  // long tiles read fewer inputs twice, short ones give more threads: 8 tokens until there are 2^18 threads of 32
+  const int TT = (long long)p.T * groups >= (1LL << 23) ? 32 : ((long long)p.T * groups >= (1LL << 22) ? 16 : 8);
   const long long tiles = (long long)p.T / TT + p.S + 2;
   const long long blocks = (tiles * groups + kConvThreads - 1) / kConvThreads;
   if (blocks > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  if (vec) return launch(causal_conv_kernel<K, 8>, dim3((unsigned)blocks), dim3(kConvThreads), 0, stream, 1, p, groups, TT, tiles);
-  return launch(causal_conv_kernel<K, 1>, dim3((unsigned)blocks), dim3(kConvThreads), 0, stream, 1, p, groups, TT, tiles);
+  return launch(causal_conv_kernel<KT, V, ES>, dim3((unsigned)blocks), dim3(kConvThreads), 0, stream, 1, p, groups, TT, tiles);
+}
+template <int KT>
+static int launch_conv(const MmbCausalConvParams& p, cudaStream_t stream) {
+  const bool vec = p.C % 4 == 0 && rows_aligned(p.x, p.ldx, p.xt, 4) && rows_aligned(p.out, p.ldo, p.ot, 4);
+  if (p.xt == 2) return vec ? launch_conv_v<KT, 4, 4>(p, stream) : launch_conv_v<KT, 1, 4>(p, stream);
+  return vec ? launch_conv_v<KT, 4, 2>(p, stream) : launch_conv_v<KT, 1, 2>(p, stream);
 }
 
-template <int K, int V>
+template <int KT, int V, int ES>
 static int launch_conv_step_v(const MmbCausalConvParams& p, cudaStream_t stream) {
   const int groups = p.C / V;
   const unsigned gx = (unsigned)((groups + kConvThreads - 1) / kConvThreads);
   const bool many = (long long)groups * p.T >= (1 << 17);
   const long long gy = many ? ((long long)p.T + 3) / 4 : p.T;
   if (gy > 65535) return (int)cudaErrorInvalidValue;
-  if (many) return launch(causal_conv_step_kernel<K, V, 4>, dim3(gx, (unsigned)gy), dim3(kConvThreads), 0, stream, 1, p, groups);
-  return launch(causal_conv_step_kernel<K, V, 1>, dim3(gx, (unsigned)gy), dim3(kConvThreads), 0, stream, 1, p, groups);
+  if (many) return launch(causal_conv_step_kernel<KT, V, ES, 4>, dim3(gx, (unsigned)gy), dim3(kConvThreads), 0, stream, 1, p, groups);
+  return launch(causal_conv_step_kernel<KT, V, ES, 1>, dim3(gx, (unsigned)gy), dim3(kConvThreads), 0, stream, 1, p, groups);
 }
-template <int K>
+template <int KT>
 static int launch_conv_step(const MmbCausalConvParams& p, cudaStream_t stream) {
   const bool vec = p.C % 4 == 0 && rows_aligned(p.x, p.ldx, p.xt, 4) && rows_aligned(p.out, p.ldo, p.ot, 4) &&
                    reinterpret_cast<uintptr_t>(p.state) % 16 == 0;
-  return vec ? launch_conv_step_v<K, 4>(p, stream) : launch_conv_step_v<K, 1>(p, stream);
+  if (p.xt == 2) return vec ? launch_conv_step_v<KT, 4, 4>(p, stream) : launch_conv_step_v<KT, 1, 4>(p, stream);
+  return vec ? launch_conv_step_v<KT, 4, 2>(p, stream) : launch_conv_step_v<KT, 1, 2>(p, stream);
 }
 
 }  // namespace mmb
@@ -224,31 +268,23 @@ static int launch_conv_step(const MmbCausalConvParams& p, cudaStream_t stream) {
 MMB_API int mmb_causal_conv(const MmbCausalConvParams* pp, cudaStream_t stream) {
   const MmbCausalConvParams& p = *pp;
   if (p.T <= 0 || p.C <= 0) return 0;
-  if (p.S < 0 || p.cu_seqlens == nullptr) return (int)cudaErrorInvalidValue;
+  if (p.S < 0 || p.cu_seqlens == nullptr || p.K < 2 || p.K > 8) return (int)cudaErrorInvalidValue;
   switch (p.K) {
     case 2: return mmb::launch_conv<2>(p, stream);
     case 3: return mmb::launch_conv<3>(p, stream);
     case 4: return mmb::launch_conv<4>(p, stream);
-    case 5: return mmb::launch_conv<5>(p, stream);
-    case 6: return mmb::launch_conv<6>(p, stream);
-    case 7: return mmb::launch_conv<7>(p, stream);
-    case 8: return mmb::launch_conv<8>(p, stream);
-    default: return (int)cudaErrorInvalidValue;
+    default: return mmb::launch_conv<8>(p, stream);
   }
 }
 
 MMB_API int mmb_causal_conv_step(const MmbCausalConvParams* pp, cudaStream_t stream) {
   const MmbCausalConvParams& p = *pp;
   if (p.T <= 0 || p.C <= 0) return 0;
-  if (p.state == nullptr) return (int)cudaErrorInvalidValue;
+  if (p.state == nullptr || p.K < 2 || p.K > 8) return (int)cudaErrorInvalidValue;
   switch (p.K) {
     case 2: return mmb::launch_conv_step<2>(p, stream);
     case 3: return mmb::launch_conv_step<3>(p, stream);
     case 4: return mmb::launch_conv_step<4>(p, stream);
-    case 5: return mmb::launch_conv_step<5>(p, stream);
-    case 6: return mmb::launch_conv_step<6>(p, stream);
-    case 7: return mmb::launch_conv_step<7>(p, stream);
-    case 8: return mmb::launch_conv_step<8>(p, stream);
-    default: return (int)cudaErrorInvalidValue;
+    default: return mmb::launch_conv_step<8>(p, stream);
   }
 }

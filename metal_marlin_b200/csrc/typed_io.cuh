@@ -78,6 +78,50 @@ __device__ __forceinline__ void stv(void* p, long long i, int t, const float* v)
     }
   }
 }
+// The same in two halves: raw bits first, so that a batch of loads is in flight before the first conversion waits for its data (a branch
+// on the type around load and conversion together would wait load by load).  ES: bytes of an element; V values are V * ES / 4 words (V * ES >= 4)
+// or one half word.
+template <int V, int ES>
+struct Raw {
+  uint32_t w[V * ES >= 4 ? V * ES / 4 : 1];
+};
+template <int V, int ES>
+__device__ __forceinline__ void ld_raw(const void* p, long long i, Raw<V, ES>& r) {
+  const unsigned char* a = reinterpret_cast<const unsigned char*>(p) + i * ES;
+  if constexpr (V * ES == 2) {
+    r.w[0] = *reinterpret_cast<const uint16_t*>(a);
+  } else if constexpr (V * ES == 4) {
+    r.w[0] = *reinterpret_cast<const uint32_t*>(a);
+  } else if constexpr (V * ES == 8) {
+    const uint2 u = *reinterpret_cast<const uint2*>(a);
+    r.w[0] = u.x, r.w[1] = u.y;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V * ES / 16; ++j) {
+      const uint4 u = reinterpret_cast<const uint4*>(a)[j];
+      r.w[4 * j] = u.x, r.w[4 * j + 1] = u.y, r.w[4 * j + 2] = u.z, r.w[4 * j + 3] = u.w;
+    }
+  }
+}
+template <int V, int ES>
+__device__ __forceinline__ void cvt_raw(const Raw<V, ES>& r, int t, float* v) {
+  if constexpr (ES == 4) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = __uint_as_float(r.w[i]);
+  } else if constexpr (V == 1) {
+    v[0] = t == 0 ? __uint_as_float(r.w[0] << 16) : __half2float(__ushort_as_half((unsigned short)r.w[0]));
+  } else {
+    unpack16<V>(r.w, t, v);
+  }
+}
+
+__device__ __forceinline__ uint32_t bits1(const void* p, long long i, int t) {
+  return t == 2 ? reinterpret_cast<const uint32_t*>(p)[i] : reinterpret_cast<const uint16_t*>(p)[i];
+}
+__device__ __forceinline__ float value1(uint32_t w, int t) {
+  return t == 0 ? __uint_as_float(w << 16) : t == 1 ? __half2float(__ushort_as_half((unsigned short)w)) : __uint_as_float(w);
+}
+
 // Whether rows of a [*, n] tensor can be read or written in pieces of `v` values.
 inline bool rows_aligned(const void* p, long long ld, int t, int v) {
   const int bytes = v * elt_bytes(t) < 16 ? v * elt_bytes(t) : 16;
