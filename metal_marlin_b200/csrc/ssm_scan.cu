@@ -4,22 +4,23 @@
 //   out_t = (sum_n h_t[n] C_t[n] + D[c] x_t) silu(z_t)
 // with h fp32 in state[row, c, 0 .. N - 1], read when a sequence starts (zero when it is fresh) and written when it ends.
 //
-// Prompts.  Every step of every state takes one exponential and four fp32 multiply-adds; at 16 exponentials a clock and SM the special
-// function unit bounds the scan (N = 16 and 16-bit activations: 3 x longer than moving the activations through memory).  The recurrence is
-// one multiply-add deep, so a warp with a few states a lane already keeps that unit busy; the work is therefore split over channels and over
-// the STATES of a channel, never over time (a second pass over time would double the exponentials).  S lanes share a channel, each with NPL
-// states in registers; 128 threads own 128 / S channels of one sequence and walk it in tiles of TT = 8 S tokens (1024 values):
-//   * the tile's x, dt, z, B, C arrive raw in shared memory by 16-byte cp.async, one tile ahead;
-//   * every thread turns 8 values into (d, d x) pairs, so softplus is paid once per value, not once per lane;
-//   * the warps scan: per token one broadcast pair and NPL values of B and C each;
-//   * partial outputs of S tokens are summed over the S lanes by a transposing butterfly (S - 1 shuffles for S tokens) that leaves every
-//     lane with the sum of one token;
-//   * every thread adds the skip term, applies the gate and stores its 8 values.
+// Prompts.  Every step of every state takes one exponential and four fp32 operations; at 16 exponentials a clock and SM the special function
+// unit bounds the scan (16 states, 16-bit activations: 3 x longer than moving the activations through memory), closely followed by the
+// 32 bytes a clock that shared memory returns to each scheduler's registers (8 bytes of B and C a state).  The recurrence itself is one
+// multiply-add deep.  The work is split over channels and over the STATES of a channel, never over time (a second pass over time would
+// double the exponentials): S lanes share a channel, each with NPL states in registers (of R channels where there are lanes to spare).  A block
+// owns 128 / S R channels of one sequence and walks it in tiles of 32 tokens with two roles that meet at named barriers, tile by tile:
+//   * four staging warps: the tile's x, dt, z, B, C arrive raw by 16-byte cp.async two tiles ahead; they turn x and dt into (d, d x) pairs, so softplus
+//     is paid once per value and not once per lane, and later add the skip term, apply the gate and store the outputs;
+//   * four scanning warps: G tokens at a time, all their exponentials before the recurrence, the next group's loads before both; partial sums of S
+//     tokens are added over the S lanes by a transposing butterfly (S - 1 shuffles for S tokens) that leaves every lane with the sum of one token.
+// What it took (4096 tokens of 8192 channels, 16 states, bf16): one role with runtime types 1132 us; blocks spread evenly over the SMs and loads of a
+// batch issued before their conversions 772 -> 547; types at compile time, conflict-free staging 386; the two roles 327; groups of four
+// tokens, unrolled 262 us.
 // exp(d A) is taken as 2^(d (A log2 e)); A log2 e is rounded once, which shifts every exponent by the same relative 2^-24.
 //
-// Single tokens.  The state is the traffic: S lanes move a channel's N values in 16-byte pieces, RB rows at a time so that A stays in registers.
+// Single tokens.  The state is the traffic: see ssm_step_kernel.
 #include <atomic>
-#include <cstdlib>
 
 #include "api_ext.h"
 #include "launch.h"
@@ -27,7 +28,8 @@
 
 namespace mmb {
 
-constexpr int kSsmThreads = 128;
+constexpr int kSsmThreads = 128;            // of each role
+constexpr int kSsmTokens = 32;              // of a tile
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -81,24 +83,91 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Sums v[i] over the S lanes of a group for i < S; lane s of the group ends with the sum of v[s] in v[0].
-template <int S>
-__device__ __forceinline__ void transposed_sum(float (&v)[S], int s) {
+// Sums v[i] over the S lanes of a group for i < S; lane s of the group ends with the sums of v[s] in v[0].
+template <int S, int R>
+__device__ __forceinline__ void transposed_sum(float (&v)[S][R], int s) {
 #pragma unroll
   for (int m = S / 2; m >= 1; m >>= 1) {
     const bool up = s & m;
 #pragma unroll
-    for (int i = 0; i < m; ++i) {
-      const float send = up ? v[i] : v[i + m], keep = up ? v[i + m] : v[i];
-      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, m);
-    }
+    for (int i = 0; i < m; ++i)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float send = up ? v[i][r] : v[i + m][r], keep = up ? v[i + m][r] : v[i][r];
+        v[i][r] = keep + __shfl_xor_sync(0xffffffffu, send, m);
+      }
   }
 }
 
-// Byte offsets of the parts of a block's shared memory; two raw stages, then the fp32 tiles.
+__device__ __forceinline__ void ld2(const void* p, int i, int t, float* v) {
+  if (t == 2) {
+    const float2 f = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p) + i);
+    v[0] = f.x, v[1] = f.y;
+  } else {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(p) + i);
+    unpack16<2>(&w, t, v);
+  }
+}
+__device__ __forceinline__ void st2(void* p, long long i, int t, const float* v) {
+  if (t == 2) *reinterpret_cast<float2*>(reinterpret_cast<float*>(p) + i) = make_float2(v[0], v[1]);
+  else *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p) + i) = pack16(v[0], v[1], t);
+}
+
+// N consecutive floats of shared memory, N a power of two or less than five, by the widest loads.
+template <int N>
+__device__ __forceinline__ void lds(const float* p, float* v) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const float4 f = reinterpret_cast<const float4*>(p)[i];
+      v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+    }
+  } else if constexpr (N == 2) {
+    const float2 f = *reinterpret_cast<const float2*>(p);
+    v[0] = f.x, v[1] = f.y;
+  } else {
+    v[0] = *p;
+  }
+}
+// Partial sums of SG tokens: SG / S times S tokens are summed over the S lanes of a channel, lane s stores token s of them.
+template <int S, int R, int SG, int YS>
+__device__ __forceinline__ void emit(float (&v)[SG][R], int s, float* yt) {
+#pragma unroll
+  for (int k = 0; k < SG; k += S) {
+    float w[S][R];
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+      for (int r = 0; r < R; ++r) w[i][r] = v[k + i][r];
+    transposed_sum<S, R>(w, s);
+    float* y = yt + k * YS;
+    if constexpr (R == 4) *reinterpret_cast<float4*>(y) = make_float4(w[0][0], w[0][1], w[0][2], w[0][3]);
+    else if constexpr (R == 2) *reinterpret_cast<float2*>(y) = make_float2(w[0][0], w[0][1]);
+    else *y = w[0][0];
+  }
+}
+
+template <int V>
+struct Int {
+  static constexpr int value = V;
+};
+
+// Pair j of a lane's NPL consecutive values, by 16-byte loads where they are.
+template <int NPL>
+__device__ __forceinline__ f32x2 at2(const float* p, int j) {
+  if constexpr (NPL % 4 == 0) {
+    const ulonglong2 u = reinterpret_cast<const ulonglong2*>(p)[j / 2];
+    return j % 2 ? u.y : u.x;
+  } else {
+    return reinterpret_cast<const f32x2*>(p)[j];
+  }
+}
+
+// Byte offsets of the parts of a block's shared memory.
 struct SsmLayout {
   int x, dt, z, b, c, stage, step, bf, cf, y, total;
 };
+constexpr int kSsmStages = 3;               // raw tiles: one arriving, one being prepared, one whose outputs are being finished
 __host__ __device__ inline SsmLayout ssm_layout(int TT, int CH, int NP, int xb, int dtb, int zb, int bb) {
   SsmLayout l;
   int at = 0;
@@ -108,20 +177,34 @@ __host__ __device__ inline SsmLayout ssm_layout(int TT, int CH, int NP, int xb, 
   l.b = at, at += TT * NP * bb;             // rows padded to NP values
   l.c = at, at += TT * NP * bb;
   l.stage = at;
-  at *= 2;
-  l.step = at, at += TT * CH * 16;          // {d, d, d x, d x}: both halves of the packed factors in one load
-  l.bf = at, at += bb == 4 ? 0 : TT * NP * 4;   // fp32 tiles are used where they arrive
-  l.cf = at, at += bb == 4 ? 0 : TT * NP * 4;
-  l.y = at, at += TT * (CH + 8) * 4;        // the padding spreads the tokens that a warp writes at once over the banks
+  at *= kSsmStages;
+  // two of each of the following
+  l.step = at, at += 2 * TT * CH * 8;       // {d, d x}
+  l.bf = at, at += bb == 4 ? 0 : 2 * TT * NP * 4;   // fp32 tiles are used where they arrive
+  l.cf = at, at += bb == 4 ? 0 : 2 * TT * NP * 4;
+  l.y = at, at += 2 * TT * (CH + 8) * 4;    // the padding spreads the tokens that a warp writes at once over the banks
   l.total = at;
   return l;
 }
 
-template <int S, int NPL>
-__global__ void __launch_bounds__(kSsmThreads) ssm_scan_kernel(const MmbSsmParams p, int n_blocks, int vec_x, int vec_bc, int vec_out) {
-  constexpr int CH = kSsmThreads / S, TT = 8 * S, NP = S * NPL, YS = CH + 8;
+// Named barriers with constant numbers (a number in a register makes a block reserve all sixteen).  Full and done: one per buffer.
+enum { kBarStage = 1, kBarFull = 2, kBarDone = 4 };
+template <int ID, int N>
+__device__ __forceinline__ void bar_sync() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
+template <int ID, int N>
+__device__ __forceinline__ void bar_arrive() { asm volatile("bar.arrive %0, %1;" ::"n"(ID), "n"(N) : "memory"); }
+template <int ID, int N>
+__device__ __forceinline__ void bar_sync_of(int buffer) { buffer ? bar_sync<ID + 1, N>() : bar_sync<ID, N>(); }
+template <int ID, int N>
+__device__ __forceinline__ void bar_arrive_of(int buffer) { buffer ? bar_arrive<ID + 1, N>() : bar_arrive<ID, N>(); }
+
+// XT: the type of x, dt, z, B, C and out where they have one type, else 3.
+template <int S, int NPL, int R, int G, int XT>
+__global__ void __launch_bounds__(2 * kSsmThreads) ssm_scan_kernel(const MmbSsmParams p, int n_blocks, int vec_x, int vec_bc, int vec_out) {
+  const int xt = XT < 3 ? XT : p.xt, dtt = XT < 3 ? XT : p.dtt, zt = XT < 3 ? XT : p.zt, bt = XT < 3 ? XT : p.bt, ot = XT < 3 ? XT : p.ot;
+  constexpr int CH = kSsmThreads / S * R, TT = kSsmTokens, NP = S * NPL, YS = CH + 8;
+  constexpr int SG = 2 * G > S ? 2 * G : S;                 // tokens between two sums over the lanes: an even number of groups
   extern __shared__ __align__(16) unsigned char sm[];
-  const int tid = threadIdx.x;
   const int seq = blockIdx.x / n_blocks, c0 = (blockIdx.x % n_blocks) * CH;
   auto start = [&](int s) { return min(max(p.cu_seqlens[s], 0), p.T); };
   const int begin = start(seq), end = seq < p.S ? max(begin, start(seq + 1)) : p.T;
@@ -134,257 +217,393 @@ __global__ void __launch_bounds__(kSsmThreads) ssm_scan_kernel(const MmbSsmParam
   }
   if (!live) {                                    // rows of no live sequence
     if (p.zero_dead)
-      for (long long i = tid; i < (long long)(end - begin) * CH; i += kSsmThreads) {
+      for (long long i = threadIdx.x; i < (long long)(end - begin) * CH; i += 2 * kSsmThreads) {
         const int c = c0 + (int)(i % CH);
-        if (c < p.D) st1(p.out, (begin + i / CH) * p.ldo + c, p.ot, 0.f);
+        if (c < p.D) st1(p.out, (begin + i / CH) * p.ldo + c, ot, 0.f);
       }
     return;
   }
-  const int xb = elt_bytes(p.xt), dtb = elt_bytes(p.dtt), zb = p.z ? elt_bytes(p.zt) : 0, bb = elt_bytes(p.bt), N = p.N;
+  const int xb = elt_bytes(xt), dtb = elt_bytes(dtt), zb = p.z ? elt_bytes(zt) : 0, bb = elt_bytes(bt), N = p.N;
   const SsmLayout L = ssm_layout(TT, CH, NP, xb, dtb, zb, bb);
-  float4* steps = reinterpret_cast<float4*>(sm + L.step);
-  float* bf = reinterpret_cast<float*>(sm + L.bf);
-  float* cf = reinterpret_cast<float*>(sm + L.cf);
-  float* yt = reinterpret_cast<float*>(sm + L.y);
+  const int tiles = (end - begin + TT - 1) / TT;
 
-  // rows t0 .. t0 + TT of a [*, width] tensor, `cols` of them from column `col`, into a dense [TT][cols] raw tile; zeros outside
-  auto fetch = [&](unsigned char* dst, const void* src, long long ld, int es, int col, int cols, int width, int t0, bool vec) {
-    if (vec) {
-      const int per = cols * es / 16;             // 16-byte pieces a row
-      for (int i = tid; i < TT * per; i += kSsmThreads) {
-        const int r = i / per, q = i - r * per;
-        const bool ok = t0 + r < end && col + q * 16 / es < width;
-        const char* g = reinterpret_cast<const char*>(src) + (ok ? ((long long)(t0 + r) * ld + col) * es + q * 16 : 0);
-        cp_async16(dst + i * 16, g, ok);
+  if (threadIdx.x >= kSsmThreads) {
+    // ------------------------------------------------------------------------------------------------ staging warps
+    const int tid = threadIdx.x - kSsmThreads;
+    // rows t0 .. t0 + TT of COLS columns (a power of two) of a [*, width] tensor into a dense raw tile; zeros outside.  16-byte pieces where the
+    // rows are aligned for it: a thread's pieces lie in one column of pieces, so its addresses are one pointer and a stride.
+    auto fetch16 = [&](auto cols, auto es, unsigned char* dst, const unsigned char* src, long long ld, int width, int t0) {
+      constexpr int COLS = decltype(cols)::value, ES = decltype(es)::value, PER = COLS * ES / 16, PIECES = TT * PER;
+      const int r0 = tid / PER, q = tid % PER;
+      const bool in = q * (16 / ES) < width;
+      const unsigned char* g = src + (t0 + r0) * ld * ES + q * 16;
+#pragma unroll
+      for (int k = 0; k < (PIECES + kSsmThreads - 1) / kSsmThreads; ++k) {
+        const int r = r0 + k * (kSsmThreads / PER);
+        if (PIECES % kSsmThreads == 0 || r < TT) {
+          const bool ok = in && t0 + r < end;
+          cp_async16(dst + (tid + k * kSsmThreads) * 16, ok ? g + k * (kSsmThreads / PER) * ld * ES : src, ok);
+        }
       }
-    } else {
-      for (int i = tid; i < TT * cols; i += kSsmThreads) {
-        const int r = i / cols, q = i - r * cols;
-        const bool ok = t0 + r < end && col + q < width;
-        const long long at = (long long)(t0 + r) * ld + col + q;
+    };
+    auto fetch = [&](auto cols, unsigned char* dst, const void* base, int col, long long ld, int es, int width, int t0, bool vec) {
+      constexpr int COLS = decltype(cols)::value;
+      const unsigned char* src = reinterpret_cast<const unsigned char*>(base) + (long long)col * es;
+      width -= col;
+      if (vec) {
+        if (es == 2) fetch16(cols, Int<2>{}, dst, src, ld, width, t0);
+        else fetch16(cols, Int<4>{}, dst, src, ld, width, t0);
+        return;
+      }
+      for (int i = tid; i < TT * COLS; i += kSsmThreads) {
+        const int r = i / COLS, q = i % COLS;
+        const bool ok = t0 + r < end && q < width;
+        const long long at = (long long)(t0 + r) * ld + q;
         if (es == 2) reinterpret_cast<uint16_t*>(dst)[i] = ok ? reinterpret_cast<const uint16_t*>(src)[at] : (uint16_t)0;
         else reinterpret_cast<uint32_t*>(dst)[i] = ok ? reinterpret_cast<const uint32_t*>(src)[at] : 0u;
       }
-    }
-  };
-  auto prefetch = [&](int t0, int stage) {
-    unsigned char* st = sm + stage * L.stage;
-    fetch(st + L.x, p.x, p.ldx, xb, c0, CH, p.D, t0, vec_x);
-    fetch(st + L.dt, p.dt, p.lddt, dtb, c0, CH, p.D, t0, vec_x);
-    if (p.z) fetch(st + L.z, p.z, p.ldz, zb, c0, CH, p.D, t0, vec_x);
-    fetch(st + L.b, p.B, p.ldb, bb, 0, NP, N, t0, vec_bc);
-    fetch(st + L.c, p.C, p.ldc, bb, 0, NP, N, t0, vec_bc);
-    cp_async_commit();
-  };
-  prefetch(begin, 0);
-
-  // this thread's 8 values of a tile: token vt, channels vc .. vc + 7
-  const int vt = tid * 8 / CH, vc = tid * 8 % CH;
-  float bias[8], skip[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const bool in = c0 + vc + i < p.D;
-    bias[i] = in && p.dt_bias ? p.dt_bias[c0 + vc + i] : 0.f;
-    skip[i] = in && p.Dskip ? p.Dskip[c0 + vc + i] : 0.f;
-  }
-  // this lane's states: channel ch, states s NPL .. s NPL + NPL - 1, in pairs
-  const int lane = tid & 31, s = lane % S, cl = (tid >> 5) * (32 / S) + lane / S, ch = c0 + cl;
-  f32x2 h[NPL / 2], a[NPL / 2];
-  const bool old = p.state && !(p.fresh && p.fresh[seq]);
-#pragma unroll
-  for (int j = 0; j < NPL / 2; ++j) {
-    float av[2], hv[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int n = s * NPL + 2 * j + e;
-      const bool in = ch < p.D && n < N;
-      av[e] = in ? p.A[(long long)ch * N + n] * kLog2e : 0.f;
-      hv[e] = in && old ? p.state[(row * p.D + ch) * N + n] : 0.f;
-    }
-    a[j] = pack2(av[0], av[1]);
-    h[j] = pack2(hv[0], hv[1]);
-  }
-  auto token = [&](int t) {
-    const ulonglong2 dd = *reinterpret_cast<const ulonglong2*>(steps + t * CH + cl);
-    f32x2 b[NPL / 2], c[NPL / 2];
-    const float *bp = bf + t * NP + s * NPL, *cp = cf + t * NP + s * NPL;
-    if constexpr (NPL == 2) {
-      b[0] = *reinterpret_cast<const f32x2*>(bp);
-      c[0] = *reinterpret_cast<const f32x2*>(cp);
-    } else {
-#pragma unroll
-      for (int j = 0; j < NPL / 4; ++j) {
-        const ulonglong2 u = reinterpret_cast<const ulonglong2*>(bp)[j], w = reinterpret_cast<const ulonglong2*>(cp)[j];
-        b[2 * j] = u.x, b[2 * j + 1] = u.y, c[2 * j] = w.x, c[2 * j + 1] = w.y;
+    };
+    auto prefetch = [&](int i) {
+      if (i < tiles) {
+        const int t0 = begin + i * TT;
+        unsigned char* st = sm + i % kSsmStages * L.stage;
+        fetch(Int<CH>{}, st + L.x, p.x, c0, p.ldx, xb, p.D, t0, vec_x);
+        fetch(Int<CH>{}, st + L.dt, p.dt, c0, p.lddt, dtb, p.D, t0, vec_x);
+        if (p.z) fetch(Int<CH>{}, st + L.z, p.z, c0, p.ldz, zb, p.D, t0, vec_x);
+        fetch(Int<NP>{}, st + L.b, p.B, 0, p.ldb, bb, N, t0, vec_bc);
+        fetch(Int<NP>{}, st + L.c, p.C, 0, p.ldc, bb, N, t0, vec_bc);
       }
-    }
-    f32x2 acc = 0;
+      cp_async_commit();
+    };
+    prefetch(0);
+    prefetch(1);
+    // this thread's values of a tile: channels vc, vc + 1 of the tokens vt, vt + VS, ..
+    constexpr int VS = 2 * kSsmThreads / CH, VN = TT / VS;
+    const int vt = tid / (CH / 2), vc = tid % (CH / 2) * 2;
+    float bias[2], skip[2];
 #pragma unroll
-    for (int j = 0; j < NPL / 2; ++j) {
-      const float2 x = unpack2(mul2(dd.x, a[j]));
-      h[j] = fma2(pack2(exp2_fast(x.x), exp2_fast(x.y)), h[j], mul2(dd.y, b[j]));
-      acc = j ? fma2(h[j], c[j], acc) : mul2(h[j], c[j]);
+    for (int i = 0; i < 2; ++i) {
+      const bool in = c0 + vc + i < p.D;
+      bias[i] = in && p.dt_bias ? p.dt_bias[c0 + vc + i] : 0.f;
+      skip[i] = in && p.Dskip ? p.Dskip[c0 + vc + i] : 0.f;
     }
-    const float2 y = unpack2(acc);
-    return y.x + y.y;
-  };
-
-  int stage = 0;
-  for (int t0 = begin; t0 < end; t0 += TT, stage ^= 1) {
-    const int valid = min(TT, end - t0);
-    unsigned char* st = sm + stage * L.stage;
-    cp_async_wait<0>();
-    __syncthreads();                              // the raw tile is there; everybody is done with the other stage and the fp32 tiles
-    if (t0 + TT < end) prefetch(t0 + TT, stage ^ 1);
-    {
-      float x[8], d[8];
-      ldv<8>(st + L.x, tid * 8, p.xt, x);
-      ldv<8>(st + L.dt, tid * 8, p.dtt, d);
+    // tile i: (d, d x) and fp32 B, C into buffer i & 1
+    auto prepare = [&](int i) {
+      const unsigned char* st = sm + i % kSsmStages * L.stage;
+      float x[VN][2], d[VN][2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) d[i] += bias[i];
+      for (int k = 0; k < VN; ++k) {
+        ld2(st + L.x, (vt + k * VS) * CH + vc, xt, x[k]);
+        ld2(st + L.dt, (vt + k * VS) * CH + vc, dtt, d[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < VN; ++k) d[k][0] += bias[0], d[k][1] += bias[1];
       if (p.softplus) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = softplus(d[i]);
+        for (int k = 0; k < VN; ++k) d[k][0] = softplus(d[k][0]), d[k][1] = softplus(d[k][1]);
       }
-      float4* dst = steps + tid * 8;
+      float4* step = reinterpret_cast<float4*>(sm + L.step + (i & 1) * TT * CH * 8);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) dst[i] = make_float4(d[i], d[i], d[i] * x[i], d[i] * x[i]);
-      if (bb == 4) {
-        bf = reinterpret_cast<float*>(st + L.b);
-        cf = reinterpret_cast<float*>(st + L.c);
-      } else {
-        for (int i = tid; i < TT * NP / 4; i += kSsmThreads) {
+      for (int k = 0; k < VN; ++k) step[((vt + k * VS) * CH + vc) / 2] = make_float4(d[k][0], d[k][0] * x[k][0], d[k][1], d[k][1] * x[k][1]);
+      if (bb == 2) {
+        float4* bf = reinterpret_cast<float4*>(sm + L.bf) + (i & 1) * TT * NP / 4;
+        float4* cf = reinterpret_cast<float4*>(sm + L.cf) + (i & 1) * TT * NP / 4;
+        for (int q = tid; q < TT * NP / 4; q += kSsmThreads) {
           float v[4];
-          ldv<4>(st + L.b, 4 * i, p.bt, v);
-          reinterpret_cast<float4*>(bf)[i] = make_float4(v[0], v[1], v[2], v[3]);
-          ldv<4>(st + L.c, 4 * i, p.bt, v);
-          reinterpret_cast<float4*>(cf)[i] = make_float4(v[0], v[1], v[2], v[3]);
+          ldv<4>(st + L.b, 4 * q, bt, v);
+          bf[q] = make_float4(v[0], v[1], v[2], v[3]);
+          ldv<4>(st + L.c, 4 * q, bt, v);
+          cf[q] = make_float4(v[0], v[1], v[2], v[3]);
         }
       }
-    }
-    __syncthreads();
-    for (int g = 0; g < valid; g += S) {
-      float v[S];
-      if (g + S <= valid) {
+    };
+    // tile i: skip term, gate, output
+    auto finish = [&](int i) {
+      const unsigned char* st = sm + i % kSsmStages * L.stage;
+      const float* yt = reinterpret_cast<const float*>(sm + L.y) + (i & 1) * TT * YS;
+      const int t0 = begin + i * TT;
+      float x[VN][2], y[VN][2];
 #pragma unroll
-        for (int i = 0; i < S; ++i) v[i] = token(g + i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < S; ++i) v[i] = g + i < valid ? token(g + i) : 0.f;
+      for (int k = 0; k < VN; ++k) {
+        ld2(st + L.x, (vt + k * VS) * CH + vc, xt, x[k]);
+        const float2 f = *reinterpret_cast<const float2*>(yt + (vt + k * VS) * YS + vc);
+        y[k][0] = f.x, y[k][1] = f.y;
       }
-      transposed_sum<S>(v, s);
-      yt[(g + s) * YS + cl] = v[0];
-    }
-    __syncthreads();
-    if (vt < valid) {
-      float x[8], y[8];
-      ldv<8>(st + L.x, tid * 8, p.xt, x);
-      ldv<8>(yt, vt * YS + vc, 2, y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = fmaf(skip[i], x[i], y[i]);
+      for (int k = 0; k < VN; ++k) y[k][0] = fmaf(skip[0], x[k][0], y[k][0]), y[k][1] = fmaf(skip[1], x[k][1], y[k][1]);
       if (p.z) {
-        float z[8];
-        ldv<8>(st + L.z, tid * 8, p.zt, z);
+        float z[VN][2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] *= silu(z[i]);
+        for (int k = 0; k < VN; ++k) ld2(st + L.z, (vt + k * VS) * CH + vc, zt, z[k]);
+#pragma unroll
+        for (int k = 0; k < VN; ++k) y[k][0] *= silu(z[k][0]), y[k][1] *= silu(z[k][1]);
       }
-      const long long at = (long long)(t0 + vt) * p.ldo + c0 + vc;
-      if (vec_out) {
-        if (c0 + vc < p.D) stv<8>(p.out, at, p.ot, y);
-      } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (c0 + vc + i < p.D) st1(p.out, at + i, p.ot, y[i]);
+      for (int k = 0; k < VN; ++k) {
+        if (t0 + vt + k * VS < end) {
+          const long long at = (long long)(t0 + vt + k * VS) * p.ldo + c0 + vc;
+          if (vec_out) {
+            if (c0 + vc < p.D) st2(p.out, at, ot, y[k]);
+          } else {
+            if (c0 + vc < p.D) st1(p.out, at, ot, y[k][0]);
+            if (c0 + vc + 1 < p.D) st1(p.out, at + 1, ot, y[k][1]);
+          }
+        }
+      }
+    };
+    for (int i = 0; i < tiles; ++i) {
+      cp_async_wait<1>();
+      bar_sync<kBarStage, kSsmThreads>();           // raw tile i is there
+      prepare(i);
+      bar_arrive_of<kBarFull, 2 * kSsmThreads>(i & 1);
+      if (i > 0) {
+        bar_sync_of<kBarDone, 2 * kSsmThreads>((i - 1) & 1);
+        finish(i - 1);
+      }
+      bar_sync<kBarStage, kSsmThreads>();           // everybody is done with raw tile i - 1
+      prefetch(i + 2);
+    }
+    bar_sync_of<kBarDone, 2 * kSsmThreads>((tiles - 1) & 1);
+    finish(tiles - 1);
+    return;
+  }
+
+  // -------------------------------------------------------------------------------------------------- scanning warps
+  // This lane: channels c0 + cl .. + R - 1, states s NPL .. s NPL + NPL - 1 of each.  The loads of the next G tokens are issued before the
+  // exponentials of these, so that one warp alone keeps the special function unit busy.
+  const int tid = threadIdx.x, lane = tid & 31, s = lane % S, cl = ((tid >> 5) * (32 / S) + lane / S) * R;
+  float h[R][NPL], a[R][NPL];
+  const bool old = p.state && !(p.fresh && p.fresh[seq]);
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) {
+      const int n = s * NPL + j, ch = c0 + cl + r;
+      const bool in = ch < p.D && n < N;
+      a[r][j] = in ? p.A[(long long)ch * N + n] * kLog2e : 0.f;
+      h[r][j] = in && old ? p.state[(row * p.D + ch) * N + n] : 0.f;
+    }
+  struct Loaded {
+    float d[G][R][2], b[G][NPL], c[G][NPL];
+  };
+  auto load = [&](const float2* step, const float* bp, const float* cp, int t, Loaded& v) {
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      lds<2 * R>(reinterpret_cast<const float*>(step + (t + g) * CH), &v.d[g][0][0]);
+      lds<NPL>(bp + (t + g) * NP, v.b[g]);
+      lds<NPL>(cp + (t + g) * NP, v.c[g]);
+    }
+  };
+  // `n` of the G loaded tokens are there
+  auto advance = [&](const Loaded& v, int n, float (*out)[R]) {
+    float e[G][R][NPL];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) e[g][r][j] = exp2_fast(v.d[g][r][0] * a[r][j]);
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        out[g][r] = 0.f;
+        if (g < n) {
+          if constexpr (NPL % 2 == 0) {
+            f32x2 acc = 0;
+#pragma unroll
+            for (int j = 0; j < NPL; j += 2) {
+              const f32x2 u = pack2(v.d[g][r][1] * v.b[g][j], v.d[g][r][1] * v.b[g][j + 1]);
+              const f32x2 hn = fma2(pack2(e[g][r][j], e[g][r][j + 1]), pack2(h[r][j], h[r][j + 1]), u);
+              const f32x2 c = pack2(v.c[g][j], v.c[g][j + 1]);
+              acc = j ? fma2(hn, c, acc) : mul2(hn, c);
+              const float2 f = unpack2(hn);
+              h[r][j] = f.x, h[r][j + 1] = f.y;
+            }
+            const float2 y = unpack2(acc);
+            out[g][r] = y.x + y.y;
+          } else {
+#pragma unroll
+            for (int j = 0; j < NPL; ++j) {
+              h[r][j] = fmaf(e[g][r][j], h[r][j], v.d[g][r][1] * v.b[g][j]);
+              out[g][r] = j ? fmaf(h[r][j], v.c[g][j], out[g][r]) : h[r][j] * v.c[g][j];
+            }
+          }
+        }
+      }
+  };
+  for (int i = 0; i < tiles; ++i) {
+    const int valid = min(TT, end - begin - i * TT);
+    const float2* step = reinterpret_cast<const float2*>(sm + L.step + (i & 1) * TT * CH * 8) + cl;
+    const float* bp = (bb == 4 ? reinterpret_cast<const float*>(sm + i % kSsmStages * L.stage + L.b) : reinterpret_cast<const float*>(sm + L.bf) + (i & 1) * TT * NP) + s * NPL;
+    const float* cp = (bb == 4 ? reinterpret_cast<const float*>(sm + i % kSsmStages * L.stage + L.c) : reinterpret_cast<const float*>(sm + L.cf) + (i & 1) * TT * NP) + s * NPL;
+    float* yt = reinterpret_cast<float*>(sm + L.y) + (i & 1) * TT * YS + s * YS + cl;
+    bar_sync_of<kBarFull, 2 * kSsmThreads>(i & 1);
+    if (valid == TT) {
+      Loaded ld[2];
+      load(step, bp, cp, 0, ld[0]);
+#pragma unroll
+      for (int t = 0; t < TT; t += SG) {
+        float v[SG][R];
+#pragma unroll
+        for (int k = 0; k < SG; k += G) {
+          if (k + G < SG || t + SG < TT) load(step, bp, cp, t + k + G, ld[(k / G + 1) & 1]);
+          advance(ld[(k / G) & 1], G, v + k);
+        }
+        emit<S, R, SG, YS>(v, s, yt + t * YS);
+      }
+    } else {
+      for (int t = 0; t < valid; t += SG) {
+        float v[SG][R];
+#pragma unroll
+        for (int k = 0; k < SG; k += G) {
+          Loaded ld;
+          load(step, bp, cp, t + k, ld);
+          advance(ld, valid - t - k, v + k);
+        }
+        emit<S, R, SG, YS>(v, s, yt + t * YS);
       }
     }
+    bar_arrive_of<kBarDone, 2 * kSsmThreads>(i & 1);
   }
   if (p.state) {
 #pragma unroll
-    for (int j = 0; j < NPL / 2; ++j) {
-      const float2 v = unpack2(h[j]);
-      const int n = s * NPL + 2 * j;
-      if (ch < p.D && n < N) p.state[(row * p.D + ch) * N + n] = v.x;
-      if (ch < p.D && n + 1 < N) p.state[(row * p.D + ch) * N + n + 1] = v.y;
-    }
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) {
+        const int n = s * NPL + j, ch = c0 + cl + r;
+        if (ch < p.D && n < N) p.state[(row * p.D + ch) * N + n] = h[r][j];
+      }
   }
 }
 
-// S lanes a channel, each PCS pieces of VEC states (4: 16 bytes), RB rows.
-template <int S, int VEC, int PCS, int RB>
-__global__ void __launch_bounds__(kSsmThreads) ssm_step_kernel(const MmbSsmParams p) {
+// One row's inputs of the single-token kernel as raw bits.  XT: the type of x, dt, z, B and C where they have one type and whole pieces can be
+// loaded, else 3; a choice at run time around every load would keep the loads from being issued together.
+template <int PCS, int XT>
+struct StepRow {
+  float h[PCS][4];
+  uint32_t b[PCS][XT < 2 ? 2 : 4], c[PCS][XT < 2 ? 2 : 4], x, dt, z;
+};
+template <int XT, int W>
+__device__ __forceinline__ void ld_quad(const void* p, long long i, int n, int t, uint32_t (&w)[W]) {
+  if constexpr (XT < 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + i);
+    w[0] = u.x, w[1] = u.y;
+  } else if constexpr (XT == 2) {
+    const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + i);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+  } else {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) w[v] = v < n ? bits1(p, i + v, t) : 0u;
+  }
+}
+template <int XT, int W>
+__device__ __forceinline__ void quad_values(const uint32_t (&w)[W], int t, float (&v)[4]) {
+  if constexpr (XT < 2) {
+    unpack16<4>(w, XT, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = XT == 2 ? __uint_as_float(w[e]) : value1(w[e], t);
+  }
+}
+template <int XT>
+__device__ __forceinline__ uint32_t ld_bits(const void* p, long long i, int t) {
+  if constexpr (XT < 2) return reinterpret_cast<const uint16_t*>(p)[i];
+  if constexpr (XT == 2) return reinterpret_cast<const uint32_t*>(p)[i];
+  return bits1(p, i, t);
+}
+
+// S lanes a channel, each PCS pieces of four states; a block owns `per` neighbouring groups of channels of one row.  What bounds it is the state
+// (read and written once); what keeps it from the memory's rate is the work around it, softplus, gate and sums, which every lane of a channel
+// repeats: two pieces a lane instead of one are worth 78 -> 51 us together with the walk along the row (256 rows of 8192 channels, 16 states: 5.6 TB/s;
+// walking the rows of one group of channels with A in registers instead, 65 us: the accesses of neighbouring blocks lie further apart).
+template <int S, int PCS, int XT>
+__global__ void __launch_bounds__(kSsmThreads) ssm_step_kernel(const MmbSsmParams p, int per) {
+  const int xt = XT < 3 ? XT : p.xt, dtt = XT < 3 ? XT : p.dtt, zt = XT < 3 ? XT : p.zt, bt = XT < 3 ? XT : p.bt;
+  constexpr int CB = kSsmThreads / S;
+  const int lane = threadIdx.x % S, N = p.N, t = blockIdx.y;
+  const int ch0 = blockIdx.x * per * CB + threadIdx.x / S;
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x % S, ch = blockIdx.x * (kSsmThreads / S) + threadIdx.x / S, N = p.N;
-  const bool in = ch < p.D;
-  const int r0 = blockIdx.y * RB;
-  long long row[RB];
-#pragma unroll
-  for (int r = 0; r < RB; ++r) row[r] = r0 + r < p.T ? pool_row(p.rows, r0 + r, p.pool_rows, p.status) : -1;
-  float h[RB][PCS][VEC], a[PCS][VEC];
-#pragma unroll
-  for (int r = 0; r < RB; ++r)
-#pragma unroll
-    for (int i = 0; i < PCS; ++i) {
-      const int n = (i * S + lane) * VEC;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) h[r][i][v] = 0.f;
-      if (in && n < N && row[r] >= 0) ldv<VEC>(p.state, (row[r] * p.D + ch) * N + n, 2, h[r][i]);
-    }
+  const long long row = pool_row(p.rows, t, p.pool_rows, p.status);
+  if (row < 0) {
+    if (p.zero_dead)
+      for (int k = 0; k < per; ++k)
+        if (ch0 + k * CB < p.D && lane == 0) st1(p.out, (long long)t * p.ldo + ch0 + k * CB, p.ot, 0.f);
+    return;
+  }
+  float b[PCS][4], c[PCS][4];
 #pragma unroll
   for (int i = 0; i < PCS; ++i) {
-    const int n = (i * S + lane) * VEC;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) a[i][v] = 0.f;
-    if (in && n < N) ldv<VEC>(p.A, (long long)ch * N + n, 2, a[i]);
+    const int n = (i * S + lane) * 4;
+    uint32_t bw[XT < 2 ? 2 : 4] = {}, cw[XT < 2 ? 2 : 4] = {};
+    if (n < N) {
+      ld_quad<XT>(p.B, (long long)t * p.ldb + n, N - n, bt, bw);
+      ld_quad<XT>(p.C, (long long)t * p.ldc + n, N - n, bt, cw);
+    }
+    quad_values<XT>(bw, bt, b[i]);
+    quad_values<XT>(cw, bt, c[i]);
   }
-  const float bias = in && p.dt_bias ? p.dt_bias[ch] : 0.f, skip = in && p.Dskip ? p.Dskip[ch] : 0.f;
-  // everything of the rows in flight before the first conversion waits for its data
-  uint32_t xr[RB], dr[RB], zr[RB], br[RB][PCS][VEC], cr[RB][PCS][VEC];
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    const long long t = r0 + r;
-    if (!in || row[r] < 0) continue;
-    xr[r] = bits1(p.x, t * p.ldx + ch, p.xt);
-    dr[r] = bits1(p.dt, t * p.lddt + ch, p.dtt);
-    if (p.z) zr[r] = bits1(p.z, t * p.ldz + ch, p.zt);
+  struct In {
+    float h[PCS][4], a[PCS][4], bias, skip;
+    uint32_t x, dt, z;
+  };
+  auto load = [&](int ch, In& q) {
 #pragma unroll
     for (int i = 0; i < PCS; ++i) {
-      const int n = (i * S + lane) * VEC;
+      const int n = (i * S + lane) * 4;
       if (n < N) {
+        const float *hs = p.state + (row * p.D + ch) * N + n, *as = p.A + (long long)ch * N + n;
+        if constexpr (XT < 3) {
+          const float4 f = *reinterpret_cast<const float4*>(hs), g = *reinterpret_cast<const float4*>(as);
+          q.h[i][0] = f.x, q.h[i][1] = f.y, q.h[i][2] = f.z, q.h[i][3] = f.w;
+          q.a[i][0] = g.x, q.a[i][1] = g.y, q.a[i][2] = g.z, q.a[i][3] = g.w;
+        } else {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) br[r][i][v] = bits1(p.B, t * p.ldb + n + v, p.bt), cr[r][i][v] = bits1(p.C, t * p.ldc + n + v, p.bt);
+          for (int v = 0; v < 4; ++v) q.h[i][v] = n + v < N ? hs[v] : 0.f, q.a[i][v] = n + v < N ? as[v] : 0.f;
+        }
       }
     }
-  }
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    const int t = r0 + r;
-    if (row[r] < 0) {
-      if (p.zero_dead && t < p.T && in && lane == 0) st1(p.out, (long long)t * p.ldo + ch, p.ot, 0.f);
-      continue;
-    }
-    const float x = in ? value1(xr[r], p.xt) : 0.f;
-    float d = in ? value1(dr[r], p.dtt) + bias : 0.f;
+    q.dt = ld_bits<XT>(p.dt, (long long)t * p.lddt + ch, dtt);
+    q.x = ld_bits<XT>(p.x, (long long)t * p.ldx + ch, xt);
+    if (p.z) q.z = ld_bits<XT>(p.z, (long long)t * p.ldz + ch, zt);
+    q.bias = p.dt_bias ? p.dt_bias[ch] : 0.f;
+    q.skip = p.Dskip ? p.Dskip[ch] : 0.f;
+  };
+  for (int k = 0; k < per; ++k) {
+    const int ch = ch0 + k * CB;
+    const bool in = ch < p.D;
+    In v;
+    if (in) load(ch, v);
+    const float x = in ? value1(v.x, xt) : 0.f;
+    float d = in ? value1(v.dt, dtt) + v.bias : 0.f;
     if (p.softplus) d = softplus(d);
     const float dx = d * x, dl = d * kLog2e;
     float acc = 0.f;
 #pragma unroll
     for (int i = 0; i < PCS; ++i) {
-      const int n = (i * S + lane) * VEC;
+      const int n = (i * S + lane) * 4;
       if (in && n < N) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          h[r][i][v] = fmaf(exp2_fast(dl * a[i][v]), h[r][i][v], dx * value1(br[r][i][v], p.bt));
-          acc = fmaf(h[r][i][v], value1(cr[r][i][v], p.bt), acc);
+        for (int e = 0; e < 4; ++e) {
+          v.h[i][e] = fmaf(exp2_fast(dl * v.a[i][e]), v.h[i][e], dx * b[i][e]);
+          if (XT < 3 || n + e < N) acc = fmaf(v.h[i][e], c[i][e], acc);
         }
-        stv<VEC>(p.state, (row[r] * p.D + ch) * N + n, 2, h[r][i]);
+        float* dst = p.state + (row * p.D + ch) * N + n;
+        if constexpr (XT < 3) {
+          *reinterpret_cast<float4*>(dst) = make_float4(v.h[i][0], v.h[i][1], v.h[i][2], v.h[i][3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < N) dst[e] = v.h[i][e];
+        }
       }
     }
 #pragma unroll
     for (int m = S / 2; m >= 1; m >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, m);
     if (in && lane == 0) {
-      float y = fmaf(skip, x, acc);
-      if (p.z) y *= silu(value1(zr[r], p.zt));
+      float y = fmaf(v.skip, x, acc);
+      if (p.z) y *= silu(value1(v.z, zt));
       st1(p.out, (long long)t * p.ldo + ch, p.ot, y);
     }
   }
@@ -402,34 +621,51 @@ static int allow_smem(F kernel, int bytes, std::atomic<unsigned long long>& done
   return (int)e;
 }
 
-template <int S, int NPL>
-static int launch_scan(const MmbSsmParams& p, cudaStream_t stream) {
-  constexpr int CH = kSsmThreads / S, TT = 8 * S;
+template <int S, int NPL, int R, int G, int XT>
+static int launch_scan_t(const MmbSsmParams& p, cudaStream_t stream) {
+  constexpr int CH = kSsmThreads / S * R, TT = kSsmTokens;
   const bool vx = p.D % 8 == 0 && rows_aligned(p.x, p.ldx, p.xt, 8) && rows_aligned(p.dt, p.lddt, p.dtt, 8) && rows_aligned(p.z, p.ldz, p.zt, 8);
   const bool vb = (p.N * elt_bytes(p.bt)) % 16 == 0 && rows_aligned(p.B, p.ldb, p.bt, 8) && rows_aligned(p.C, p.ldc, p.bt, 8);
-  const bool vo = p.D % 8 == 0 && rows_aligned(p.out, p.ldo, p.ot, 8);
+  const bool vo = p.D % 2 == 0 && rows_aligned(p.out, p.ldo, p.ot, 2);
   const int nb = (p.D + CH - 1) / CH;
   const long long blocks = (long long)nb * (p.S + 1);
   if (blocks > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  const SsmLayout L = ssm_layout(TT, CH, S * NPL, elt_bytes(p.xt), elt_bytes(p.dtt), p.z ? elt_bytes(p.zt) : 0, elt_bytes(p.bt));
+  size_t smem = ssm_layout(TT, CH, S * NPL, elt_bytes(p.xt), elt_bytes(p.dtt), p.z ? elt_bytes(p.zt) : 0, elt_bytes(p.bt)).total;
+  // a grid of a few blocks a SM is not spread evenly by itself: ask for so much shared memory that no SM takes more than its share
+  constexpr int kSmem = 227 * 1024;
+  const long long share = ((long long)nb * p.S + 147) / 148;
+  if (share >= 1 && share <= 4) smem = max(smem, (size_t)(kSmem / share - 1024) / 128 * 128);
   static std::atomic<unsigned long long> done{0};
-  // the largest this instance can ask for: fp32 activations, all of its states
-  const int e = allow_smem(ssm_scan_kernel<S, NPL>, ssm_layout(TT, CH, S * NPL, 4, 4, 4, 4).total, done);
+  const int e = allow_smem(ssm_scan_kernel<S, NPL, R, G, XT>, kSmem, done);
   if (e) return e;
   // not a programmatic dependent launch: blocks that start while the previous kernel drains pile up on the SMs that it leaves first, and a scan
-  // has too few blocks to even that out (4096 tokens, 8192 channels back to back: 1132 us against 837 us for a lone one, first version)
-  ssm_scan_kernel<S, NPL><<<(unsigned)blocks, kSsmThreads, (size_t)L.total, stream>>>(p, nb, (int)vx, (int)vb, (int)vo);
+  // has too few blocks to even that out
+  ssm_scan_kernel<S, NPL, R, G, XT><<<(unsigned)blocks, 2 * kSsmThreads, smem, stream>>>(p, nb, (int)vx, (int)vb, (int)vo);
   return (int)cudaGetLastError();
 }
+template <int S, int NPL, int R, int G>
+static int launch_scan(const MmbSsmParams& p, cudaStream_t stream) {
+  const bool same = p.dtt == p.xt && p.bt == p.xt && p.ot == p.xt && (p.z == nullptr || p.zt == p.xt);
+  if (!same) return launch_scan_t<S, NPL, R, G, 3>(p, stream);
+  return p.xt == 0 ? launch_scan_t<S, NPL, R, G, 0>(p, stream) : p.xt == 1 ? launch_scan_t<S, NPL, R, G, 1>(p, stream) : launch_scan_t<S, NPL, R, G, 2>(p, stream);
+}
 
-template <int S, int VEC, int PCS>
+template <int S, int PCS, int XT>
+static int launch_step_t(const MmbSsmParams& p, cudaStream_t stream) {
+  const int groups = (p.D + kSsmThreads / S - 1) / (kSsmThreads / S);
+  // a few groups of channels a block share its row's B and C, while that leaves eight blocks for every SM
+  int per = 1;
+  while (per < 4 && (long long)p.T * ((groups + 2 * per - 1) / (2 * per)) >= 8 * 148) per *= 2;
+  if (p.T > 65535) return (int)cudaErrorInvalidValue;
+  return launch(ssm_step_kernel<S, PCS, XT>, dim3((unsigned)((groups + per - 1) / per), (unsigned)p.T), dim3(kSsmThreads), 0, stream, 1, p, per);
+}
+template <int S, int PCS>
 static int launch_step(const MmbSsmParams& p, cudaStream_t stream) {
-  const unsigned gx = (unsigned)((p.D + kSsmThreads / S - 1) / (kSsmThreads / S));
-  const bool many = (long long)gx * p.T >= 8192;
-  const long long gy = many ? ((long long)p.T + 1) / 2 : p.T;
-  if (gy > 65535) return (int)cudaErrorInvalidValue;
-  if (many) return launch(ssm_step_kernel<S, VEC, PCS, 2>, dim3(gx, (unsigned)gy), dim3(kSsmThreads), 0, stream, 1, p);
-  return launch(ssm_step_kernel<S, VEC, PCS, 1>, dim3(gx, (unsigned)gy), dim3(kSsmThreads), 0, stream, 1, p);
+  const bool vec = p.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.state) % 16 == 0 && reinterpret_cast<uintptr_t>(p.A) % 16 == 0 &&
+                   rows_aligned(p.B, p.ldb, p.bt, 4) && rows_aligned(p.C, p.ldc, p.bt, 4) && p.dtt == p.xt && p.bt == p.xt &&
+                   (p.z == nullptr || p.zt == p.xt);
+  if (!vec) return launch_step_t<S, PCS, 3>(p, stream);
+  return p.xt == 0 ? launch_step_t<S, PCS, 0>(p, stream) : p.xt == 1 ? launch_step_t<S, PCS, 1>(p, stream) : launch_step_t<S, PCS, 2>(p, stream);
 }
 
 }  // namespace mmb
@@ -438,21 +674,26 @@ MMB_API int mmb_ssm_scan(const MmbSsmParams* pp, cudaStream_t stream) {
   const MmbSsmParams& p = *pp;
   if (p.T <= 0 || p.D <= 0) return 0;
   if (p.S < 0 || p.N < 1 || p.N > 128 || p.cu_seqlens == nullptr) return (int)cudaErrorInvalidValue;
-  const char* ev = getenv("SSM_V"); const int v = ev ? atoi(ev) : 0;
-  if (p.N <= 8) return mmb::launch_scan<4, 2>(p, stream);
-  if (p.N <= 16) return v == 1 ? mmb::launch_scan<2, 8>(p, stream) : v == 2 ? mmb::launch_scan<8, 2>(p, stream) : mmb::launch_scan<4, 4>(p, stream);
-  if (p.N <= 32) return mmb::launch_scan<8, 4>(p, stream);
-  if (p.N <= 64) return mmb::launch_scan<8, 8>(p, stream);
-  return mmb::launch_scan<8, 16>(p, stream);
+  // Lanes a channel: few while there are blocks for every SM, more when a warp would be alone on its scheduler.  Measured (bf16, 16 states; us for
+  // S = 4 / 8 / 16): 4096 tokens of 8192 channels 264 / 350 / 394, 2048 of 2560 92 / 90 / 92, 4096 of 1536 178 / 129 / 133, 2000 of 512 90 / 68 / 54.
+  const long long width = (long long)p.D * (p.S > 0 ? p.S : 1);
+  if (p.N <= 8) return width >= 4096 ? mmb::launch_scan<4, 2, 1, 4>(p, stream) : mmb::launch_scan<8, 1, 1, 4>(p, stream);
+  if (p.N <= 16) {
+    if (width >= 4096) return mmb::launch_scan<4, 4, 1, 4>(p, stream);
+    return width >= 1024 ? mmb::launch_scan<8, 2, 1, 4>(p, stream) : mmb::launch_scan<16, 1, 1, 2>(p, stream);
+  }
+  if (p.N <= 32) return mmb::launch_scan<8, 4, 1, 4>(p, stream);
+  // 64 states: two channels a lane halve the shared memory reads of B and C (2000 tokens of 4096 channels, bf16: 199 us against 248 us) once there are
+  // enough lanes for it (1531 tokens of 1536 channels, fp32: 117 us against 94 us)
+  if (p.N <= 64) return width >= 4096 ? mmb::launch_scan<16, 4, 2, 1>(p, stream) : mmb::launch_scan<16, 4, 1, 4>(p, stream);
+  return mmb::launch_scan<16, 8, 1, 2>(p, stream);
 }
 
 MMB_API int mmb_ssm_step(const MmbSsmParams* pp, cudaStream_t stream) {
   const MmbSsmParams& p = *pp;
   if (p.T <= 0 || p.D <= 0) return 0;
   if (p.N < 1 || p.N > 128 || p.state == nullptr) return (int)cudaErrorInvalidValue;
-  const bool vec = p.N % 4 == 0 && reinterpret_cast<uintptr_t>(p.state) % 16 == 0 && reinterpret_cast<uintptr_t>(p.A) % 16 == 0;
-  if (vec && p.N <= 16) return mmb::launch_step<4, 4, 1>(p, stream);
-  if (vec && p.N <= 32) return mmb::launch_step<8, 4, 1>(p, stream);
-  if (vec) return mmb::launch_step<16, 4, 2>(p, stream);
-  return p.N <= 32 ? mmb::launch_step<16, 1, 2>(p, stream) : mmb::launch_step<16, 1, 8>(p, stream);
+  if (p.N <= 16) return mmb::launch_step<2, 2>(p, stream);
+  if (p.N <= 32) return mmb::launch_step<4, 2>(p, stream);
+  return p.N <= 64 ? mmb::launch_step<8, 2>(p, stream) : mmb::launch_step<8, 4>(p, stream);
 }
