@@ -5,17 +5,26 @@
 // 4 flops a query head and cached value, 1 to 16 heads a value: bound by the bytes of the visible K and V rows.
 //
 // Split.  The visible keys of one (sequence, KV head) are cut over the CTAs of a cluster, theirs over four warps, and each warp walks tiles of 16
-// keys on its own: a private ring of tiles filled by 16-byte cp.async straight from the pages, no block barrier inside the loop.  Every warp keeps
-// a running maximum and sum (fp32, base 2) and an O accumulator in registers; the warps are joined in shared memory and the CTAs through
+// or 32 keys on its own: a private ring of tiles filled by 16-byte cp.async straight from the pages, no block barrier inside the loop.  Every warp
+// keeps a reference maximum and a sum (fp32, base 2) and an O accumulator in registers; the warps are joined in shared memory and the CTAs through
 // distributed shared memory in the same launch.  No global workspace: captured graphs share nothing and no result depends on arrival order.
+// The reference of a row moves only when a score exceeds it by more than 2^8 (one vote for all rows; the usual tile has no shuffles).
 //
 // Tensor cores (m16n8k16): all query heads of a KV head are the rows of one product, so a key is read once.
 //   S = Q K^T: the contraction may be permuted, so a lane reads 8 consecutive values (16 bytes of bf16) of its key and uses them as the B
 //   fragments of two k-steps; Q is held in the same order.
 //   O = P V: the output columns may be permuted, so a lane reads 8 consecutive columns of its four keys and pairs them up with byte permutes.
-// P is split into two bf16 numbers (P = hi + lo to 2^-17): a single bf16 P would add as much error as rounding the output does.  Up to 8 heads fill
-// only half of the 16 rows; hi and lo then take rows 0-7 and 8-15 of ONE product.  9 to 16 heads take two products.
-// Quantized pools: the codes are exact in bf16; the row scale of K multiplies the score and that of V the probability, both in fp32.
+// P is split into two 16-bit numbers (P = hi + lo to 2^-17): a single bf16 P would add as much error as rounding the output does.  Up to 8 heads
+// fill only half of the 16 rows; hi and lo then take rows 0-7 and 8-15 of ONE product.  9 to 16 heads take two products.
+//
+// Quantized pools: the codes of every format are exact in f16, so both products run in f16.  Q goes in divided by a power of two per row, undone in
+// the score; the row scale of K multiplies the score and that of V the probability, both in fp32.  Probabilities times value scales are kept in f16's
+// range by a reference for the scales (4 x the largest seen) and a factor of 2^7.
+//
+// Measured (graph replays, heads 32 / 8 of 128, window 4096 + 4, three input sets in turn): 64 rows bf16 164 us = 6.5 TB/s, the measured copy rate;
+// 8 rows 26 us; 1 row 11.5 us.  int8 32 rows 64 us and fp8 64 rows 141 us, 1.5 to 1.7 x the time of their bytes: half the bytes a key, the
+// same instructions a key plus the conversions, so the issue slots bound them (hardware conversions into f16 instead of bf16: int8 117 -> 76 us;
+// 32 keys a tile 76 -> 64).
 #include <atomic>
 #include <cuda_fp4.h>
 
@@ -25,21 +34,23 @@
 
 namespace mmb {
 
-constexpr int kSdWarps = 4, kSdThreads = kSdWarps * 32, kSdTile = 16;
+constexpr float kSdLazy = 8.f;              // log2 units
+constexpr int kSdWarps = 4, kSdThreads = kSdWarps * 32;
 
 enum { kSdBf16 = 0, kSdFp8 = 1, kSdInt8 = 2, kSdFp4 = 3, kSdInt4 = 4 };
 
 template <int D, int F>
 struct SdCfg {
   static constexpr int row_bytes = F == kSdBf16 ? D * 2 : (F <= kSdInt8 ? D : D / 2);
+  static constexpr int T = F == kSdBf16 || D == 256 ? 16 : 32;          // keys a tile
   static constexpr int U = row_bytes / 16;                       // 16-byte units a row
   static constexpr int piece = row_bytes * 8 / D;                // bytes of 8 values
-  static constexpr int tile_bytes = 2 * kSdTile * row_bytes;     // K and V
-  static constexpr int scale_bytes = F == kSdBf16 ? 0 : 2 * kSdTile * 4;
+  static constexpr int tile_bytes = 2 * T * row_bytes;     // K and V
+  static constexpr int scale_bytes = F == kSdBf16 ? 0 : 2 * T * 4;
   static constexpr int stage_bytes = tile_bytes + scale_bytes;
-  // as many stages as fit next to a second CTA on the SM, at least three
-  static constexpr int fit = (100 * 1024) / (kSdWarps * stage_bytes);
-  static constexpr int NST = fit < 3 ? 3 : (fit > 6 ? 6 : fit);
+  // as many stages as fit next to two more CTAs on the SM, two to four (more stages and fewer CTAs were slower: the warps, not the copies, are short)
+  static constexpr int fit = (72 * 1024) / (kSdWarps * stage_bytes);
+  static constexpr int NST = fit < 2 ? 2 : (fit > 4 ? 4 : fit);
   static constexpr int ring_bytes = kSdWarps * NST * stage_bytes;
 };
 
@@ -67,44 +78,64 @@ __device__ __forceinline__ uint32_t sd_pack(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 8 cached values at `p` as four bf16 pairs.
+// 8 cached codes at `p` as four f16 pairs (all formats are exact in it).  int8: 0x6400 + u is the f16 number 1024 + u for 0 <= u < 256.
 template <int F>
-__device__ __forceinline__ void sd_load8(const unsigned char* p, uint32_t (&w)[4]) {
-  if constexpr (F == kSdBf16) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-  } else if constexpr (F == kSdFp8) {
+__device__ __forceinline__ void sd_load8_f16(const unsigned char* p, uint32_t (&w)[4]) {
+  if constexpr (F == kSdFp8) {
     const uint2 u = *reinterpret_cast<const uint2*>(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __nv_fp8x2_storage_t c = (__nv_fp8x2_storage_t)((i < 2 ? u.x : u.y) >> (16 * (i & 1)));
-      const __half2 h = __half2(__nv_cvt_fp8x2_to_halfraw2(c, __NV_E4M3));
-      const float2 f = __half22float2(h);
-      w[i] = sd_pack(f.x, f.y);
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((i < 2 ? u.x : u.y) >> (16 * (i & 1))), __NV_E4M3);
+      w[i] = (uint32_t)h.x | (uint32_t)h.y << 16;
     }
   } else if constexpr (F == kSdInt8) {
     const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int c = (int)((i < 2 ? u.x : u.y) >> (16 * (i & 1)));
-      w[i] = sd_pack((float)(signed char)(c & 0xff), (float)(signed char)((c >> 8) & 0xff));
+      const uint32_t m = __byte_perm((i < 2 ? u.x : u.y) ^ 0x80808080u, 0x64646464u, i & 1 ? 0x4342 : 0x4140);
+      const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&m), off);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
   } else if constexpr (F == kSdFp4) {
     const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __half2 h = __half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((u >> (8 * i)) & 0xff), __NV_E2M1));
-      const float2 f = __half22float2(h);
-      w[i] = sd_pack(f.x, f.y);
+      const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((u >> (8 * i)) & 0xff), __NV_E2M1);
+      w[i] = (uint32_t)h.x | (uint32_t)h.y << 16;
     }
   } else {
-    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(p) ^ 0x88888888u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6408));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int lo = (int)(u << (28 - 8 * i)) >> 28, hi = (int)(u << (24 - 8 * i)) >> 28;
-      w[i] = sd_pack((float)lo, (float)hi);
+      const uint32_t n = u >> (8 * i);
+      const uint32_t m = (n & 0xfu) | (n & 0xf0u) << 12 | 0x64006400u;
+      const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&m), off);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
   }
+}
+template <int F>
+__device__ __forceinline__ void sd_load8(const unsigned char* p, uint32_t (&w)[4]) {
+  if constexpr (F == kSdBf16) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+  } else {
+    sd_load8_f16<F>(p, w);
+  }
+}
+template <int N>
+__device__ __forceinline__ float sd_max(const float (&v)[N]) {
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
+  return m;
+}
+template <int F>
+__device__ __forceinline__ void sd_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (F == kSdBf16) mma_bf16_16816(d, a0, a1, a2, a3, b0, b1);
+  else mma_f16_16816(d, a0, a1, a2, a3, b0, b1);
 }
 
 __device__ __forceinline__ void sd_cp16(void* dst, const void* src, bool ok) {
@@ -135,14 +166,15 @@ __device__ __forceinline__ float4 sd_remote_f4(uint32_t addr) {
 
 // grid (splits, Hkv * head groups, B), clusters of `splits`.  WIDE: 16 query heads a CTA, else 8.
 template <int D, int F, bool WIDE>
-__global__ void __launch_bounds__(kSdThreads) sink_decode_kernel(const MmbSinkDecodeParams p, int splits, int head_groups, int bs_shift) {
+__global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSinkDecodeParams p, int splits, int head_groups, int bs_shift) {
   using Cfg = SdCfg<D, F>;
-  constexpr int R = WIDE ? 16 : 8, U = Cfg::U, NST = Cfg::NST, NI = D / 32, NJ = D / 64;
+  constexpr int R = WIDE ? 16 : 8, U = Cfg::U, NST = Cfg::NST, NI = D / 32, NJ = D / 64, T = Cfg::T, NT = T / 8, KT = T / 16;
   constexpr bool kScaled = F != kSdBf16;
   extern __shared__ __align__(16) unsigned char sm[];
   __shared__ __align__(16) unsigned char q_sm[R * D * 2];        // 16-byte pieces, placed like the units of K
   __shared__ float ml[kSdWarps][R][2], ml_cta[R][2];
   __shared__ unsigned ok_sm[kSdWarps][NST];
+  __shared__ float q_scale[R];
   pdl_launch_dependents();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
@@ -152,9 +184,9 @@ __global__ void __launch_bounds__(kSdThreads) sink_decode_kernel(const MmbSinkDe
   // visible keys: j < n_sink at position j, the others at position j + shift
   const int n = max(0, (int)min((long long)p.ctx_lens[b], (long long)p.max_blocks * p.block_size));
   const int lo = max(0, n - p.window), n_sink = min(p.sinks, lo), shift = lo - n_sink, m = n - shift;
-  const int per = ((m + splits - 1) / splits + kSdTile - 1) / kSdTile * kSdTile;
+  const int per = ((m + splits - 1) / splits + T - 1) / T * T;
   const int j_begin = min(m, rank * per), j_end = min(m, j_begin + per);
-  const int tiles = (j_end - j_begin + kSdTile - 1) / kSdTile;
+  const int tiles = (j_end - j_begin + T - 1) / T;
   const int mine = tiles > warp ? (tiles - warp + kSdWarps - 1) / kSdWarps : 0;
 
   for (int i = tid; i < R * D / 8; i += kSdThreads) {
@@ -164,50 +196,83 @@ __global__ void __launch_bounds__(kSdThreads) sink_decode_kernel(const MmbSinkDe
     *reinterpret_cast<uint4*>(q_sm + (r * (D / 8) + (c ^ ((r & 1) << 2))) * 16) = v;
   }
   __syncthreads();
+  if constexpr (kScaled) {
+    // f16 products take q divided by the power of two at its row's largest magnitude (nothing below 2^-24 of that matters to a score)
+    for (int r = warp; r < R; r += kSdWarps) {
+      bf16* row = reinterpret_cast<bf16*>(q_sm) + r * D;
+      float m = 0.f;
+      for (int i = lane; i < D; i += 32) m = fmaxf(m, fabsf(__bfloat162float(row[i])));
+      m = warp_max(m);
+      const int e = m > 0.f && m < INFINITY ? (int)(__float_as_uint(m) >> 23) - 127 : 0;
+      const int half_e = e / 2;                                   // two factors: 2^-e alone can overflow
+      const float f0 = __uint_as_float((uint32_t)(127 - half_e) << 23), f1 = __uint_as_float((uint32_t)(127 - (e - half_e)) << 23);
+      for (int i = lane; i < D; i += 32) reinterpret_cast<__half*>(row)[i] = __float2half_rn(__bfloat162float(row[i]) * f0 * f1);
+      if (lane == 0) q_scale[r] = 1.f / f0 / f1;
+    }
+    __syncthreads();
+  }
 
+  const long long row_stride = (long long)p.Hkv * Cfg::row_bytes;
+  const int head_at = hk * Cfg::row_bytes;
   unsigned char* ring = sm + warp * NST * Cfg::stage_bytes;
   const int* table = p.block_tables + (long long)b * p.max_blocks;
-  // cache slot of key `lane % 16` of tile t of this warp, -1 where there is none
-  auto slot_of = [&](int t) -> long long {
-    const int j = j_begin + (warp + t * kSdWarps) * kSdTile + (lane & 15);
+  // cache slot of key `lane % T` of tile t of this warp, -1 where there is none
+  auto slot_of = [&](int t) -> int {
+    const int j = j_begin + (warp + t * kSdWarps) * T + lane % T;
     if (t >= mine || j >= j_end) return -1;
     const int pos = j < n_sink ? j : j + shift;
     const int blk = bs_shift >= 0 ? pos >> bs_shift : pos / p.block_size;
     const long long slot = (long long)table[blk] * p.block_size + (pos - blk * p.block_size);
-    if (slot >= 0 && slot < p.n_slots) return slot;
+    if (slot >= 0 && slot < p.n_slots) return (int)slot;
     if (p.status) atomicExch(p.status, 131);
     return -1;
   };
-  auto issue = [&](int t, long long slot) {
+  auto issue = [&](int t, int slot) {
     if (t < mine) {
       unsigned char* st = ring + (t % NST) * Cfg::stage_bytes;
-      const unsigned ok = __ballot_sync(0xffffffffu, slot >= 0) & 0xffffu;
+      const unsigned ok = __ballot_sync(0xffffffffu, slot >= 0);
       if (lane == 0) ok_sm[warp][t % NST] = ok;
 #pragma unroll
-      for (int i = 0; i < kSdTile * U / 32; ++i) {
+      for (int i = 0; i < T * U / 32; ++i) {
         const int e = i * 32 + lane, r = e / U, u = e % U;
-        const long long sl = __shfl_sync(0xffffffffu, slot, r);
-        const long long at = sl >= 0 ? (sl * p.Hkv + hk) * Cfg::row_bytes + u * 16 : 0;
+        const int sl = __shfl_sync(0xffffffffu, slot, r);
+        const long long at = (long long)max(sl, 0) * row_stride + (head_at + u * 16);
         sd_cp16(st + (r * U + sd_unit_k<U, Cfg::piece>(r, u)) * 16, reinterpret_cast<const unsigned char*>(p.k) + at, sl >= 0);
         sd_cp16(st + Cfg::tile_bytes / 2 + (r * U + sd_unit_v<U, Cfg::piece>(r, u)) * 16, reinterpret_cast<const unsigned char*>(p.v) + at, sl >= 0);
       }
       if constexpr (kScaled) {
-        const long long at = slot >= 0 ? slot * p.Hkv + hk : 0;
-        sd_cp4(st + Cfg::tile_bytes + lane * 4, (lane < 16 ? p.k_scale : p.v_scale) + at, slot >= 0);
+        const long long at = slot >= 0 ? (long long)slot * p.Hkv + hk : 0;
+        if constexpr (T == 16) {
+          sd_cp4(st + Cfg::tile_bytes + lane * 4, (lane < 16 ? p.k_scale : p.v_scale) + at, slot >= 0);
+        } else {
+          sd_cp4(st + Cfg::tile_bytes + lane * 4, p.k_scale + at, slot >= 0);
+          sd_cp4(st + Cfg::tile_bytes + (T + lane) * 4, p.v_scale + at, slot >= 0);
+        }
       }
     }
     sd_commit();
   };
 
+  constexpr bool kQReg = D <= 128;
+  uint4 qr[kQReg ? NI : 1][WIDE ? 2 : 1];
+  if constexpr (kQReg) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int h = 0; h < (WIDE ? 2 : 1); ++h) qr[i][h] = *reinterpret_cast<const uint4*>(q_sm + ((gid + 8 * h) * (D / 8) + ((tig + 4 * i) ^ ((gid & 1) << 2))) * 16);
+  }
   float o[NJ * 8][4];
 #pragma unroll
   for (int i = 0; i < NJ * 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float v_ref = 0.f;                                             // quantized: reference of the value scales
   float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};      // rows gid and (WIDE) gid + 8
   const float c = p.scale * 1.4426950408889634f;
+  float cr[2] = {c, c};
+  if constexpr (kScaled) cr[0] = c * q_scale[gid], cr[1] = WIDE ? c * q_scale[gid + 8 * WIDE] : 0.f;
 
 #pragma unroll
   for (int t = 0; t < NST - 1; ++t) issue(t, slot_of(t));
-  long long next = slot_of(NST - 1);
+  int next = slot_of(NST - 1);
   for (int t = 0; t < mine; ++t) {
     issue(t + NST - 1, next);
     next = slot_of(t + NST);
@@ -216,99 +281,137 @@ __global__ void __launch_bounds__(kSdThreads) sink_decode_kernel(const MmbSinkDe
     const unsigned char* st = ring + (t % NST) * Cfg::stage_bytes;
     const unsigned char* vt = st + Cfg::tile_bytes / 2;
     const unsigned ok = ok_sm[warp][t % NST];
-    float s[2][4] = {};
+    float s[NT][4] = {}, s2[NT][4] = {};
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int pc = tig + 4 * i;
-      const uint4 qa = *reinterpret_cast<const uint4*>(q_sm + (gid * (D / 8) + (pc ^ ((gid & 1) << 2))) * 16);
-      uint4 qb = make_uint4(0, 0, 0, 0);
-      if constexpr (WIDE) qb = *reinterpret_cast<const uint4*>(q_sm + ((gid + 8) * (D / 8) + (pc ^ ((gid & 1) << 2))) * 16);
+      uint4 qa, qb = make_uint4(0, 0, 0, 0);
+      if constexpr (kQReg) {
+        qa = qr[i][0];
+        if constexpr (WIDE) qb = qr[i][WIDE];
+      } else {
+        qa = *reinterpret_cast<const uint4*>(q_sm + (gid * (D / 8) + (pc ^ ((gid & 1) << 2))) * 16);
+        if constexpr (WIDE) qb = *reinterpret_cast<const uint4*>(q_sm + ((gid + 8) * (D / 8) + (pc ^ ((gid & 1) << 2))) * 16);
+      }
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
+      for (int nt = 0; nt < NT; ++nt) {
         const int r = gid + 8 * nt;
         uint32_t w[4];
-        sd_load8<F>(st + (r * U + sd_unit_k<U, Cfg::piece>(r, pc * Cfg::piece / 16)) * 16 + pc * Cfg::piece % 16, w);
-        mma_bf16_16816(s[nt], qa.x, qb.x, qa.y, qb.y, w[0], w[1]);
-        mma_bf16_16816(s[nt], qa.z, qb.z, qa.w, qb.w, w[2], w[3]);
+        const unsigned char* kp = st + (r * U + sd_unit_k<U, Cfg::piece>(r, pc * Cfg::piece / 16)) * 16 + pc * Cfg::piece % 16;
+        sd_load8<F>(kp, w);
+        sd_mma<F>(s[nt], qa.x, qb.x, qa.y, qb.y, w[0], w[1]);
+        sd_mma<F>(s2[nt], qa.z, qb.z, qa.w, qb.w, w[2], w[3]);
       }
     }
-    // scores in units of log2; this lane's keys are 2 tig, 2 tig + 1 (nt 0) and 8 more (nt 1)
-    float p4[2][4];                                              // [row half][key]
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < (WIDE ? 4 : 2); ++e) s[nt][e] += s2[nt][e];
+    // scores in units of log2; this lane's keys are 8 nt + 2 tig, + 1
+    float p4[2][2 * NT];                                         // [row half][key]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int key = 8 * nt + 2 * tig + e;
-        float f = c;
-        if constexpr (kScaled) f *= reinterpret_cast<const float*>(st + Cfg::tile_bytes)[key];
+        float f = 1.f;
+        if constexpr (kScaled) f = reinterpret_cast<const float*>(st + Cfg::tile_bytes)[key];
         const bool in = ok >> key & 1;
-        p4[0][2 * nt + e] = in ? s[nt][e] * f : -INFINITY;
-        p4[1][2 * nt + e] = in ? s[nt][2 + e] * f : -INFINITY;
+        p4[0][2 * nt + e] = in ? s[nt][e] * (cr[0] * f) : -INFINITY;
+        p4[1][2 * nt + e] = in ? s[nt][2 + e] * (cr[1] * f) : -INFINITY;
       }
+    // the reference of a row moves only when one of its scores is more than kSdLazy above it; the test is one vote for all rows
     bool grew = false;
-    float alpha[2] = {1.f, 1.f};
-#pragma unroll
-    for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
-      float t4 = fmaxf(fmaxf(p4[h][0], p4[h][1]), fmaxf(p4[h][2], p4[h][3]));
-      t4 = fmaxf(t4, __shfl_xor_sync(0xffffffffu, t4, 1));
-      t4 = fmaxf(t4, __shfl_xor_sync(0xffffffffu, t4, 2));
-      if (t4 > mx[h]) {
-        alpha[h] = sd_exp2(mx[h] - t4);
-        mx[h] = t4;
-        grew = true;
-      }
-      const float ref = mx[h] == -INFINITY ? 0.f : mx[h];
-      float sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        p4[h][k] = sd_exp2(p4[h][k] - ref);
-        sum += p4[h][k];
-      }
-      l[h] = l[h] * alpha[h] + sum;
-    }
-    if (__any_sync(0xffffffffu, grew)) {
-      const float a1 = WIDE ? alpha[1] : alpha[0];
-#pragma unroll
-      for (int i = 0; i < NJ * 8; ++i) o[i][0] *= alpha[0], o[i][1] *= alpha[0], o[i][2] *= a1, o[i][3] *= a1;
-    }
+    float vs[2 * NT] = {};
     if constexpr (kScaled) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float f = reinterpret_cast<const float*>(st + Cfg::tile_bytes)[16 + 8 * (k >> 1) + 2 * tig + (k & 1)];
-        p4[0][k] *= f;
-        if constexpr (WIDE) p4[1][k] *= f;
+      for (int k = 0; k < 2 * NT; ++k) {
+        vs[k] = reinterpret_cast<const float*>(st + Cfg::tile_bytes)[T + 8 * (k >> 1) + 2 * tig + (k & 1)];
+        grew |= vs[k] > v_ref;
       }
     }
-    uint32_t hi[2][2], lw[2][2];                                 // [row half][key half]
+#pragma unroll
+    for (int h = 0; h < (WIDE ? 2 : 1); ++h) grew |= sd_max(p4[h]) > mx[h] + kSdLazy;
+    if (__any_sync(0xffffffffu, grew)) {
+      float alpha[2] = {1.f, 1.f}, beta = 1.f;
+      if constexpr (kScaled) {
+        float m = sd_max(vs);
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        if (m > v_ref) {
+          beta = v_ref / (4.f * m);
+          v_ref = 4.f * m;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
+        float t4 = sd_max(p4[h]);
+        t4 = fmaxf(t4, __shfl_xor_sync(0xffffffffu, t4, 1));
+        t4 = fmaxf(t4, __shfl_xor_sync(0xffffffffu, t4, 2));
+        if (t4 > mx[h]) {
+          alpha[h] = sd_exp2(mx[h] - t4);
+          mx[h] = t4;
+          l[h] *= alpha[h];
+        }
+      }
+      const float a0 = alpha[0] * beta, a1 = (WIDE ? alpha[1] : alpha[0]) * beta;
+#pragma unroll
+      for (int i = 0; i < NJ * 8; ++i) o[i][0] *= a0, o[i][1] *= a0, o[i][2] *= a1, o[i][3] *= a1;
+    }
+#pragma unroll
+    for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
+      const float ref = mx[h] == -INFINITY ? 0.f : mx[h];
+#pragma unroll
+      for (int k = 0; k < 2 * NT; ++k) p4[h][k] = sd_exp2(p4[h][k] - ref);
+#pragma unroll
+      for (int k = 0; k < 2 * NT; k += 4) l[h] += (p4[h][k] + p4[h][k + 1]) + (p4[h][k + 2] + p4[h][k + 3]);
+    }
+    if constexpr (kScaled) {
+      const float inv = v_ref > 0.f ? 128.f / v_ref : 0.f;
+#pragma unroll
+      for (int k = 0; k < 2 * NT; ++k) {
+        p4[0][k] *= vs[k] * inv;
+        if constexpr (WIDE) p4[1][k] *= vs[k] * inv;
+      }
+    }
+    uint32_t hi[2][NT], lw[2][NT];                               // [row half][eight keys]
 #pragma unroll
     for (int h = 0; h < (WIDE ? 2 : 1); ++h)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < NT; ++k) {
         const float x = p4[h][2 * k], y = p4[h][2 * k + 1];
-        hi[h][k] = sd_pack(x, y);
-        lw[h][k] = sd_pack(x - __uint_as_float(hi[h][k] << 16), y - __uint_as_float(hi[h][k] & 0xffff0000u));
-      }
-#pragma unroll
-    for (int jj = 0; jj < NJ; ++jj) {
-      const int pc = gid + 8 * jj;
-      uint32_t v[4][4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = 2 * tig + (k & 1) + 8 * (k >> 1);
-        sd_load8<F>(vt + (r * U + sd_unit_v<U, Cfg::piece>(r, pc * Cfg::piece / 16)) * 16 + pc * Cfg::piece % 16, v[k]);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t sel = e & 1 ? 0x7632u : 0x5410u;
-        const uint32_t b0 = __byte_perm(v[0][e >> 1], v[1][e >> 1], sel), b1 = __byte_perm(v[2][e >> 1], v[3][e >> 1], sel);
-        if constexpr (WIDE) {
-          mma_bf16_16816(o[jj * 8 + e], hi[0][0], hi[1][0], hi[0][1], hi[1][1], b0, b1);
-          mma_bf16_16816(o[jj * 8 + e], lw[0][0], lw[1][0], lw[0][1], lw[1][1], b0, b1);
+        if constexpr (kScaled) {
+          hi[h][k] = pack16(x, y, 1);
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[h][k]));
+          lw[h][k] = pack16(x - f.x, y - f.y, 1);
         } else {
-          mma_bf16_16816(o[jj * 8 + e], hi[0][0], lw[0][0], hi[0][1], lw[0][1], b0, b1);
+          hi[h][k] = sd_pack(x, y);
+          lw[h][k] = sd_pack(x - __uint_as_float(hi[h][k] << 16), y - __uint_as_float(hi[h][k] & 0xffff0000u));
         }
       }
-    }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int jj = 0; jj < NJ; ++jj) {
+        const int pc = gid + 8 * jj;
+        uint32_t v[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = 16 * kt + 2 * tig + (k & 1) + 8 * (k >> 1);
+          sd_load8<F>(vt + (r * U + sd_unit_v<U, Cfg::piece>(r, pc * Cfg::piece / 16)) * 16 + pc * Cfg::piece % 16, v[k]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t sel = e & 1 ? 0x7632u : 0x5410u;
+          const uint32_t b0 = __byte_perm(v[0][e >> 1], v[1][e >> 1], sel), b1 = __byte_perm(v[2][e >> 1], v[3][e >> 1], sel);
+          if constexpr (WIDE) {
+            sd_mma<F>(o[jj * 8 + e], hi[0][2 * kt], hi[1][2 * kt], hi[0][2 * kt + 1], hi[1][2 * kt + 1], b0, b1);
+            sd_mma<F>(o[jj * 8 + e], lw[0][2 * kt], lw[1][2 * kt], lw[0][2 * kt + 1], lw[1][2 * kt + 1], b0, b1);
+          } else {
+            sd_mma<F>(o[jj * 8 + e], hi[0][2 * kt], lw[0][2 * kt], hi[0][2 * kt + 1], lw[0][2 * kt + 1], b0, b1);
+          }
+        }
+      }
     __syncwarp();                                                // the stage may be refilled
   }
 
@@ -336,7 +439,7 @@ __global__ void __launch_bounds__(kSdThreads) sink_decode_kernel(const MmbSinkDe
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float (&x)[4] = o[jj * 8 + q * 4 + i];
-            f[i] = WIDE ? x[2 * h + e] : x[e] + x[2 + e];
+            f[i] = (WIDE ? x[2 * h + e] : x[e] + x[2 + e]) * (kScaled ? v_ref * (1.f / 128.f) : 1.f);
           }
           dst[q] = make_float4(f[0], f[1], f[2], f[3]);
         }
@@ -412,23 +515,28 @@ static int launch_sinks(const MmbSinkDecodeParams& p, cudaStream_t stream) {
   constexpr int join = kSdWarps * R * D * 4;
   constexpr int smem = Cfg::ring_bytes > join ? Cfg::ring_bytes : join;
   auto kern = sink_decode_kernel<D, F, WIDE>;
-  static std::atomic<unsigned long long> done{0};
+  // the shared memory limit and how many CTAs an SM takes belong to a device: CTAs + 1 of each, 0 = not asked yet
+  static std::atomic<int> resident[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
-  if (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1)) {       // the limit belongs to a device
+  int ctas = dev < 64 ? resident[dev].load(std::memory_order_relaxed) - 1 : -1;
+  if (ctas < 0) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kern, kSdThreads, smem);
     if (e != cudaSuccess) return (int)e;
-    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    if (dev < 64) resident[dev].store(ctas + 1, std::memory_order_relaxed);
   }
   const int G = p.Hq / p.Hkv, hg = (G + R - 1) / R;
   if ((long long)p.Hkv * hg > 65535 || p.B > 65535) return (int)cudaErrorInvalidValue;
   int splits = p.splits;
   if (splits == 0) {
     const long long most = min((long long)p.window + p.sinks, (long long)p.max_blocks * p.block_size);
-    const long long tiles = (most + kSdTile - 1) / kSdTile, rows = (long long)p.B * p.Hkv * hg;
+    const long long tiles = (most + Cfg::T - 1) / Cfg::T, rows = (long long)p.B * p.Hkv * hg;
+    // as many as the SMs hold at once: a second wave costs more than idle slots (24 rows of 8 KV heads: 1 split 74 us, 3 splits 87), a larger cluster
+    // more than it saves once the SMs are full (64 rows: 1 split 164 us, 2 splits 177, 8 splits 232)
     splits = 1;
-    while (splits < 8 && rows * splits < 2 * 148 && splits * 2 * kSdWarps <= tiles) splits *= 2;
+    while (splits < 8 && rows * (splits + 1) <= 148 * ctas && (splits + 1) * kSdWarps <= tiles) ++splits;
   }
   int shift = -1;
   if ((p.block_size & (p.block_size - 1)) == 0)
@@ -459,7 +567,7 @@ MMB_API int mmb_sink_decode(const MmbSinkDecodeParams* pp, cudaStream_t stream) 
   const MmbSinkDecodeParams& p = *pp;
   if (p.B <= 0) return 0;
   if (p.Hkv < 1 || p.Hq < 1 || p.Hq % p.Hkv != 0 || p.window < 1 || p.sinks < 0 || p.block_size < 1 || p.max_blocks < 0 || p.n_slots < 0 ||
-      (p.splits != 0 && p.splits != 1 && p.splits != 2 && p.splits != 4 && p.splits != 8))
+      p.splits < 0 || p.splits > 8)
     return (int)cudaErrorInvalidValue;
   switch (p.D) {
     case 64: return mmb::launch_sinks_f<64>(p, stream);

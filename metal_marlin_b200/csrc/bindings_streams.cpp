@@ -172,7 +172,7 @@ void sink_decode(const Tensor& q, const Tensor& k, const Tensor& v, const OptT& 
   TORCH_CHECK_VALUE(D == 64 || D == 128 || D == 256, "attention with sinks takes head sizes 64, 128 and 256, got ", D);
   TORCH_CHECK_VALUE(Hkv >= 1 && Hq >= 1 && Hq % Hkv == 0 && Hq <= INT_MAX, "query heads must be a multiple of KV heads");
   TORCH_CHECK_VALUE(block_size >= 1 && block_size <= INT_MAX, "block_size must be positive");
-  TORCH_CHECK_VALUE(splits == 0 || splits == 1 || splits == 2 || splits == 4 || splits == 8, "attention with sinks takes 1, 2, 4 or 8 splits, got ", splits);
+  TORCH_CHECK_VALUE(splits >= 0 && splits <= 8, "attention with sinks takes 1 to 8 splits, got ", splits);
   TORCH_CHECK_VALUE(q.scalar_type() == at::kBFloat16 && out.scalar_type() == at::kBFloat16, "q and out must be bf16");
   TORCH_CHECK_VALUE(q.is_contiguous() && q.numel() == B * Hq * D, "q must be contiguous with ", B * Hq * D, " values");
   TORCH_CHECK_VALUE(out.is_contiguous() && out.numel() == B * Hq * D, "out must be contiguous with ", B * Hq * D, " values");
@@ -186,6 +186,7 @@ void sink_decode(const Tensor& q, const Tensor& k, const Tensor& v, const OptT& 
                     "K and V pools must be contiguous [slots, ", Hkv, ", ", row, "]");
   MmbSinkDecodeParams p{};
   p.n_slots = k.numel() / (Hkv * row);
+  TORCH_CHECK_VALUE(p.n_slots <= INT_MAX, "the pools have too many slots");
   if (fmt >= 0) {
     p.k_scale = opt_f32(k_scale, p.n_slots * Hkv, q, "k_scale");
     p.v_scale = opt_f32(v_scale, p.n_slots * Hkv, q, "v_scale");

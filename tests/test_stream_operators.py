@@ -470,7 +470,7 @@ def test_refusals_of_attention_with_sinks():
     out = torch.empty_like(a[0])
     call = dict(q=a[0], k=a[1], v=a[2], ks=None, vs=None, tables=a[3], ctx=lens, out=out, Hq=Hq, Hkv=Hkv, D=D, bs=bs, scale=0.1, window=8, sinks=2, fmt=-1, splits=0)
     odd = torch.zeros(out.numel() + 1, dtype=torch.bfloat16)[1:].view(2, 4, 64)
-    for change in (dict(window=0), dict(window=2 ** 31), dict(sinks=-1), dict(D=32), dict(Hkv=3), dict(Hkv=0), dict(bs=0), dict(splits=3), dict(q=a[0].float()), dict(q=a[0][:1]),
+    for change in (dict(window=0), dict(window=2 ** 31), dict(sinks=-1), dict(D=32), dict(Hkv=3), dict(Hkv=0), dict(bs=0), dict(splits=9), dict(q=a[0].float()), dict(q=a[0][:1]),
                    dict(out=out.float()), dict(out=odd), dict(q=odd), dict(tables=a[3].long()), dict(tables=a[3][:1]), dict(ctx=lens.long()), dict(fmt=0), dict(fmt=5),
                    dict(k=a[1][:16]), dict(k=a[1].float(), v=a[2].float()), dict(k=a[1].view(torch.uint8)[..., :64].contiguous(), v=a[2].view(torch.uint8)[..., :64].contiguous(), fmt=0)):
         with pytest.raises(ValueError):
