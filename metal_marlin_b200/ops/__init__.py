@@ -576,14 +576,15 @@ def _sink_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv,
             out.copy_(o.view_as(out))
             return out
         return o
+    q = q.contiguous()
     if out is None:
-        out = torch.empty(B, Hq, dv, dtype=torch.bfloat16, device=q.device)
+        out = torch.empty_like(q) if q.dim() == 3 else torch.empty(B, Hq, dv, dtype=torch.bfloat16, device=q.device)
     _report_on(q.device)
     if quant:
-        K.mmb200.sink_decode(q.contiguous(), k_pool.data, v_pool.data, k_pool.scale, v_pool.scale, block_tables, ctx_lens, out, Hq, Hkv, dv, block_size,
+        K.mmb200.sink_decode(q, k_pool.data, v_pool.data, k_pool.scale, v_pool.scale, block_tables, ctx_lens, out, Hq, Hkv, dv, block_size,
                              scale, window, sinks, k_pool.fmt_code, 0)
     else:
-        K.mmb200.sink_decode(q.contiguous(), k_pool, v_pool, None, None, block_tables, ctx_lens, out, Hq, Hkv, dv, block_size, scale, window, sinks, -1, 0)
+        K.mmb200.sink_decode(q, k_pool, v_pool, None, None, block_tables, ctx_lens, out, Hq, Hkv, dv, block_size, scale, window, sinks, -1, 0)
     return out
 
 
@@ -600,7 +601,7 @@ def _report_on(device) -> None:
 def _stream_out(x, out, out_dtype, *inputs):
     """The output of a call over token rows: a new tensor, or the caller's after a check that no input of other rows lies in it."""
     if out is None:
-        return torch.empty(x.shape, dtype=out_dtype or x.dtype, device=x.device)
+        return torch.empty_like(x) if out_dtype is None else torch.empty_like(x, dtype=out_dtype)
     if out_dtype is not None and out.dtype != out_dtype:
         raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
     for t in inputs:
