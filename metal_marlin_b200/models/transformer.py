@@ -255,6 +255,8 @@ class Transformer:
         rot = cfg.qk_rope_head_dim if cfg.is_mla else cfg.dh
         self.inv_freq, self.rope_mscale = rope_inv_freq(cfg, rot, self.device)
         self.scale = cfg.softmax_scale()
+        if cfg.attention_sinks and cfg.is_mla:
+            raise ValueError("attention_sinks need per-head keys and values, not a latent (MLA) cache")
         self.mtp = None      # optional multi-token-prediction head (spec/mtp.py)
         # tensor parallelism (parallel/tp.py): a shard keeps only its local heads / vocabulary rows
         self._chain = None   # decode-chain runner (ops/chain.py); False once found unsupported for this model
@@ -304,7 +306,7 @@ class Transformer:
             qc = q.contiguous().view(T, Hq, D)
             o = ops.paged_attention(qc, kv.k[li], kv.v[li], meta.block_tables, meta.ctx_lens, Hq=Hq, Hkv=Hk, dqk=D, dv=D,
                                     block_size=kv.block_size, scale=self.scale, window=cfg.sliding_window,
-                                    splits=meta.splits, max_ctx=meta.max_ctx)
+                                    splits=meta.splits, max_ctx=meta.max_ctx, sinks=cfg.attention_sinks)
             o = o.reshape(T, Hq * D)
         else:
             o = self._prefill_attention_gqa(q.reshape(T, Hq, D), kv, li, meta)
@@ -319,6 +321,7 @@ class Transformer:
         out = torch.empty(q.shape[0], Hq * D, dtype=torch.bfloat16, device=q.device)
         bs = kv.block_size
         win = int(cfg.sliding_window or 0)
+        sinks = int(cfg.attention_sinks or 0) if win else 0      # the gathers below cut off everything in front of the window: not with sinks
 
         def _first_key(t, n_ctx):
             # with a sliding window only the keys the chunk's first query can still see are gathered
@@ -336,7 +339,7 @@ class Transformer:
                 return meta.block_tables[b, tok // bs].long() * bs + tok % bs
             return pool.view(-1, Hk, D)[meta.cached(("slots", b, lo, n_ctx), _slots)]
 
-        if (meta.attn_mask is None and q.dtype == torch.bfloat16 and len(meta.cu_seqlens) == 2 and q.stride(2) == 1
+        if (not sinks and meta.attn_mask is None and q.dtype == torch.bfloat16 and len(meta.cu_seqlens) == 2 and q.stride(2) == 1
                 and ops.fmha_ok(q.shape[0], int(meta.ctx_lens_host[0]), D, D, q.device)):
             # one long sequence: its cache rows (this chunk included) gathered once, then the tcgen05 attention kernel
             n_ctx = int(meta.ctx_lens_host[0])
@@ -345,7 +348,7 @@ class Transformer:
                              window=win)
             return out
         n_seq = len(meta.cu_seqlens) - 1
-        if (meta.attn_mask is None and q.dtype == torch.bfloat16 and n_seq > 1 and q.stride(2) == 1
+        if (not sinks and meta.attn_mask is None and q.dtype == torch.bfloat16 and n_seq > 1 and q.stride(2) == 1
                 and all(ops.fmha_ok(meta.cu_seqlens[b + 1] - meta.cu_seqlens[b], int(meta.ctx_lens_host[b]), D, D, q.device)
                         for b in range(n_seq))):
             # several long sequences: the tcgen05 attention kernel sequence by sequence (a launch per sequence costs
@@ -363,7 +366,7 @@ class Transformer:
             max_q = max(meta.cu_seqlens[i + 1] - meta.cu_seqlens[i] for i in range(len(meta.cu_seqlens) - 1))
             ops.prefill_attention(q, kv.k[li].view(-1, Hk, D), kv.v[li].view(-1, Hk, D), cu_q, block_tables=meta.block_tables,
                                   ctx_lens=meta.ctx_lens, block_size=bs, max_q=max_q, scale=self.scale, window=cfg.sliding_window,
-                                  out=out.view(-1, Hq, D))
+                                  sinks=sinks, out=out.view(-1, Hq, D))
             return out
         if (meta.attn_mask is not None and q.dtype == torch.bfloat16 and len(meta.cu_seqlens) == 2 and q.is_cuda
                 and D in ops.PREFILL_ATTN_DIMS and ops.native_available()):
@@ -391,13 +394,23 @@ class Transformer:
                 kpos = tok.unsqueeze(0)
                 mask = kpos <= qpos
                 if cfg.sliding_window:
-                    mask &= kpos > qpos - cfg.sliding_window
+                    mask &= (kpos > qpos - cfg.sliding_window) | (kpos < sinks)
             if meta.attn_mask is not None:
                 mask = meta.attn_mask
             o = F.scaled_dot_product_attention(Q, K, V, attn_mask=mask, is_causal=(mask is None), scale=self.scale,
                                                enable_gqa=(Hq != Hk))
             out[s:e] = o.squeeze(0).transpose(0, 1).reshape(t, Hq * D)
         return out
+
+    def _stream_rows(self, meta: BatchMeta, first):
+        """What the pooled-state operators need of a batch: decode ``(rows, None, None)`` with -1 for padding rows; prompts ``(rows,
+        cu_seqlens, fresh)``, a sequence being fresh when this pass holds all of its tokens."""
+        if meta.decode:
+            return torch.where(meta.slots >= 0, first, torch.full_like(first, -1)), None, None
+        cu = meta.dev_ints("cu_q", meta.cu_seqlens, first.device)
+        fresh = meta.cached("fresh", lambda: torch.tensor([int(meta.ctx_lens_host[b]) == meta.cu_seqlens[b + 1] - meta.cu_seqlens[b]
+                                                           for b in range(len(meta.cu_seqlens) - 1)], device=first.device))
+        return first[: cu.numel() - 1].contiguous(), cu, fresh
 
     def _attn_deltanet(self, L: LayerWeights, li: int, h, d, kv: PagedKVStorage, meta: BatchMeta):
         """Gated DeltaNet mixer (linear attention with the gated delta rule): ``in_proj -> causal depthwise conv + SiLU on
@@ -433,11 +446,19 @@ class Transformer:
                 q, k = q.repeat_interleave(rep, -2), k.repeat_interleave(rep, -2)
             return q, k, v
 
+        # on the device the convolution of the whole batch is one launch over the window pool
+        xc_all = None
+        if ops._use_native(proj) and 2 <= Kc <= 8:
+            rows, cu, fresh_rows = self._stream_rows(meta, meta.block_tables[:, 0].long())
+            conv = dict(state=conv_pool, rows=rows, out_dtype=torch.float32)
+            xc_all = (ops.causal_conv_step(proj[:, : 2 * kd + vd], w, **conv) if meta.decode else
+                      ops.causal_conv(proj[:, : 2 * kd + vd], w, cu_seqlens=cu, fresh=fresh_rows, **conv))
         if meta.decode:
-            win = torch.cat([conv_pool.index_select(0, first), qkv.unsqueeze(-1)], -1)            # [B, C, Kc]
-            xc = F.silu((win * w).sum(-1))
-            conv_pool.index_copy_(0, first, win[..., 1:].contiguous())
-            q, k, v = heads(xc)
+            if xc_all is None:
+                win = torch.cat([conv_pool.index_select(0, first), qkv.unsqueeze(-1)], -1)        # [B, C, Kc]
+                xc_all = F.silu((win * w).sum(-1))
+                conv_pool.index_copy_(0, first, win[..., 1:].contiguous())
+            q, k, v = heads(xc_all)
             S = state_pool.index_select(0, first)
             o = gated_delta_step(q, k, v, g, beta, S, scale=dk ** -0.5).to(torch.float32)           # [B, Hv, dv]
             state_pool.index_copy_(0, first, S)
@@ -448,10 +469,13 @@ class Transformer:
                 t = e0 - s0
                 idx = first[bi: bi + 1]
                 fresh = int(meta.ctx_lens_host[bi]) == t                                            # the sequence starts in this pass
-                hist = torch.zeros(1, 2 * kd + vd, Kc - 1, device=h.device) if fresh else conv_pool.index_select(0, idx)
-                xin = torch.cat([hist[0], qkv[s0:e0].t()], -1)                                      # [C, Kc - 1 + t]
-                xc = F.silu(F.conv1d(xin.unsqueeze(0), w.unsqueeze(1), groups=w.shape[0])[0].t())   # [t, C]
-                conv_pool.index_copy_(0, idx, xin[:, -(Kc - 1):].unsqueeze(0).contiguous())
+                if xc_all is not None:
+                    xc = xc_all[s0:e0]
+                else:
+                    hist = torch.zeros(1, 2 * kd + vd, Kc - 1, device=h.device) if fresh else conv_pool.index_select(0, idx)
+                    xin = torch.cat([hist[0], qkv[s0:e0].t()], -1)                                      # [C, Kc - 1 + t]
+                    xc = F.silu(F.conv1d(xin.unsqueeze(0), w.unsqueeze(1), groups=w.shape[0])[0].t())   # [t, C]
+                    conv_pool.index_copy_(0, idx, xin[:, -(Kc - 1):].unsqueeze(0).contiguous())
                 q, k, v = heads(xc)
                 S0 = None if fresh else state_pool.index_select(0, idx)
                 os_, S = gated_delta_rule_chunked(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), g[s0:e0].unsqueeze(0), beta[s0:e0].unsqueeze(0),
@@ -466,14 +490,15 @@ class Transformer:
     def _attn_mamba(self, L: LayerWeights, li: int, h, d, kv: PagedKVStorage, meta: BatchMeta):
         """Mamba mixer (selective state space): ``in_proj -> [x | z]``, causal depthwise conv + SiLU on x, ``x_proj -> dt, B, C``,
         ``h_t = exp(dt_t A) h_{t-1} + dt_t B_t x_t``, ``y_t = C_t h_t + D x_t``, ``y * silu(z) -> out_proj``.  Convolution window and
-        state per sequence live in ``kv.rec[li]`` like the DeltaNet state; prompt passes run the selective-scan kernel per
-        sequence, decode steps the single-step kernel.  Parity: reference ``metal_marlin/architectures/mamba.py``,
+        state per sequence live in ``kv.rec[li]`` like the DeltaNet state; on the device a prompt pass or a decode step is one convolution and
+        one scan launch for all of its sequences.  Parity: reference ``metal_marlin/architectures/mamba.py``,
         ``src/mamba_ssm.metal:204``."""
         from ..arch.mamba import selective_scan, selective_scan_step
         cfg = self.cfg
         Di, N, r, Kc = cfg.mamba_d_inner, cfg.mamba_d_state, cfg.mamba_rank, cfg.mamba_d_conv
         T = h.shape[0]
         xz, h = self._norm_linear(h, d, L.mamba_in, L.input_norm)
+        xz_in = xz
         xz = xz.to(torch.float32)
         x, z = xz[:, :Di], xz[:, Di:]
         conv_pool, state_pool = kv.rec[li]
@@ -487,6 +512,23 @@ class Transformer:
             proj = ops.linear(xc.to(torch.bfloat16).contiguous(), L.mamba_x).to(torch.float32)
             dt = F.softplus(proj[:, :r] @ L.mamba_dt.float().t() + L.mamba_dt_b.float())
             return dt, proj[:, r: r + N], proj[:, r + N: r + 2 * N]
+
+        if ops._use_native(xz_in) and 2 <= Kc <= 8 and N <= 128:
+            # on the device: the whole batch at once over the pools, one launch for the convolution and one for the scan
+            rows, cu, fresh = self._stream_rows(meta, meta.block_tables[:, 0].long())
+            D = L.mamba_D.float().contiguous()
+            if meta.decode:
+                xc = ops.causal_conv_step(xz_in[:, :Di], w, wb, state=conv_pool, rows=rows, out_dtype=torch.float32)
+                dt, Bm, Cm = ssm_inputs(xc)
+                # the roundings of the single-token path stay where they were: the convolved input and the output in bf16, then the gate
+                y = ops.ssm_step(xc.to(torch.bfloat16), dt, A, Bm, Cm, state=state_pool, rows=rows, D=D)
+                y = (y.to(torch.float32) * F.silu(z)).to(torch.bfloat16)
+            else:
+                xc = ops.causal_conv(xz_in[:, :Di], w, wb, cu_seqlens=cu, state=conv_pool, rows=rows, fresh=fresh, out_dtype=torch.float32)
+                dt, Bm, Cm = ssm_inputs(xc)
+                y = ops.ssm_scan(xc, dt, A, Bm, Cm, cu_seqlens=cu, state=state_pool, rows=rows, fresh=fresh, D=D, z=xz_in[:, Di:],
+                                 out_dtype=torch.bfloat16)
+            return h, ops.linear(y, L.mamba_out)
 
         if meta.decode:
             win = torch.cat([conv_pool.index_select(0, first), x.unsqueeze(-1)], -1)              # [B, Di, Kc]
