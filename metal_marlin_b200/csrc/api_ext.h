@@ -298,7 +298,8 @@ extern "C" {
 #endif
 // Attention of one new token per sequence over a paged pool, visible keys p < sinks or p >= ctx - window (attention_sinks.cu).  K / V pools
 // [n_slots, Hkv, D] bf16 (fmt -1) or codes with fp32 row scales [n_slots, Hkv] (fmt 0 E4M3, 1 int8, 2 E2M1, 3 int4; the 4-bit formats hold
-// the even element in the low nibble).  D is 64, 128 or 256.  A block table entry outside the pool hides its tokens and reports status 131.
+// the even element in the low nibble).  D is 64, 128 or 256.  A block table entry outside the pool hides its
+// tokens, a sequence longer than its table ends with it; both report status 131.
 typedef struct {
   const void* q;            // bf16 [B, Hq, D] contiguous
   const void* k;
@@ -312,7 +313,7 @@ typedef struct {
   long long n_slots;
   int window, sinks;        // window >= 1
   float scale;
-  int splits;               // CTAs that share a (sequence, KV head): 1, 2, 4, 8; 0 = the launcher's choice
+  int splits;               // CTAs that share a (sequence, KV head): 1 to 8; 0 = the launcher's choice
   int* status;
 } MmbSinkDecodeParams;
 int mmb_sink_decode(const MmbSinkDecodeParams* p, cudaStream_t stream);

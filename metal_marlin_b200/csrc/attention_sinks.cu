@@ -182,7 +182,9 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
   const int G = p.Hq / p.Hkv, head0 = hk * G + hg * R, heads = min(R, G - hg * R);
 
   // visible keys: j < n_sink at position j, the others at position j + shift
-  const int n = max(0, (int)min((long long)p.ctx_lens[b], (long long)p.max_blocks * p.block_size));
+  const long long room = (long long)p.max_blocks * p.block_size;
+  const int n = max(0, (int)min((long long)p.ctx_lens[b], room));
+  if (p.ctx_lens[b] > room && tid == 0 && p.status) atomicExch(p.status, 131);      // more tokens than its table has places for
   const int lo = max(0, n - p.window), n_sink = min(p.sinks, lo), shift = lo - n_sink, m = n - shift;
   const int per = ((m + splits - 1) / splits + T - 1) / T * T;
   const int j_begin = min(m, rank * per), j_end = min(m, j_begin + per);

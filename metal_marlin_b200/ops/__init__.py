@@ -514,8 +514,8 @@ def paged_attention(q, k_pool, v_pool, block_tables, ctx_lens, *, Hq, Hkv, dqk, 
     ``window > 0``: the new token sees the last ``window`` tokens of its sequence, itself included; with ``sinks > 0`` the first
     ``sinks`` tokens stay visible too (the mask of :func:`prefill_attention`).  Sinks take per-head K / V pools of any cache
     format and head sizes 64, 128 and 256; one launch splits and joins by itself (``csrc/attention_sinks.cu``), so ``splits`` and
-    ``workspace`` do not apply.  A sequence without tokens gives zeros; a block outside the pool hides its tokens and is
-    reported by :func:`check_status`."""
+    ``workspace`` do not apply.  A sequence without tokens gives zeros; a block outside the pool hides its tokens and a
+    sequence longer than its table ends with it, both reported by :func:`check_status`."""
     B = ctx_lens.numel()
     if sinks:
         if sinks < 0 or window < 0:

@@ -392,6 +392,61 @@ def test_refusals_of_the_state_operators():
         ops.ssm_step(p["x"], p["dt"], p["A"], p["Bm"], p["Cm"], state=p["state"], rows=p["rows"])
 
 
+# the launchers choose other tiles, splits of a channel and rows a block for large calls: the same definitions at sizes that reach them
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,C,dtype,out", [([2500, 0, 100], 4096, "bf16", None), ([700, 8000, 3], 4096, "fp16", "fp32"), ([4000, 300], 2050, "bf16", "bf16"),
+                                              ([90] * 40, 4096, "fp32", None)])
+def test_conv_of_large_batches(lens, C, dtype, out):
+    x, w, b, state, rows, fresh, cu = conv_inputs("cuda", lens, C, 4, TYPES[dtype], tail=5)
+    want = conv_oracle(x, w, b, state, spans(cu, fresh, rows.tolist()), 1)
+    got = ops.causal_conv(x, w, b, cu_seqlens=torch.tensor(cu, dtype=torch.int32, device="cuda"), state=state, rows=rows.to("cuda"), fresh=fresh.to("cuda"),
+                          out_dtype=TYPES[out] if out else None)
+    check_conv(got, state, *want)
+
+
+@pytest.mark.gpu
+def test_conv_of_many_short_sequences():
+    """More sequences than the kernel keeps starts of in shared memory."""
+    lens = [1 + i % 3 for i in range(1500)]
+    x, w, b, state, rows, fresh, cu = conv_inputs("cuda", lens, 12, 4, torch.bfloat16)
+    want = conv_oracle(x, w, b, state, spans(cu, fresh, rows.tolist()), 1)
+    got = ops.causal_conv(x, w, b, cu_seqlens=torch.tensor(cu, dtype=torch.int32, device="cuda"), state=state, rows=rows.to("cuda"), fresh=fresh.to("cuda"))
+    check_conv(got, state, *want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,K", [(8192, 4), (4100, 5)])
+def test_conv_of_a_large_decode_batch(C, K):
+    B = 257
+    x, w, b, _, _, _, _ = conv_inputs("cuda", [B], C, K, torch.bfloat16)
+    state = gen(9, "cuda")(B + 3, C, K - 1)
+    rows = torch.randperm(B + 3, generator=torch.Generator().manual_seed(2))[:B]
+    rows[5], rows[200] = -1, -1
+    want = conv_oracle(x, w, b, state, [(i, 1, r, False) for i, r in enumerate(rows.tolist())], 1)
+    check_conv(ops.causal_conv_step(x, w, b, state=state, rows=rows.to("cuda")), state, *want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,C,N,dtype", [([45, 3], 2104, 16, "bf16"), ([33], 4160, 16, "fp16"), ([40, 31], 2056, 7, "bf16"), ([35], 4100, 8, "fp32"),
+                                            ([37], 4104, 64, "bf16"), ([40, 9], 1032, 16, "bf16"), ([70], 4096, 30, "bf16"), ([33], 4104, 50, "fp32"), ([34], 1500, 16, "fp32")])
+def test_scan_of_wide_layers(lens, C, N, dtype):
+    p = ssm_inputs("cuda", lens, C, N, TYPES[dtype], tail=3)
+    out, state = run_ssm(p, "cuda")
+    check_ssm(out, state, want_ssm(p))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,C,N", [(80, 4100, 16), (300, 2048, 16), (70, 1000, 64), (90, 600, 128)])
+def test_scan_of_a_large_decode_batch(B, C, N):
+    p = ssm_inputs("cuda", [B], C, N, torch.bfloat16, seed=4)
+    state = gen(8, "cuda")(B + 2, C, N)
+    rows = torch.randperm(B + 2, generator=torch.Generator().manual_seed(2))[:B]
+    rows[3], rows[B - 1] = -1, -1
+    want = ssm_oracle(p["x"], p["dt"], p["A"], p["Bm"], p["Cm"], p["D"], p["z"], p["dt_bias"], True, state, [(i, 1, r, False) for i, r in enumerate(rows.tolist())])
+    out = ops.ssm_step(p["x"], p["dt"], p["A"], p["Bm"], p["Cm"], state=state, rows=rows.to("cuda"), D=p["D"], z=p["z"], dt_bias=p["dt_bias"], dt_softplus=True)
+    check_ssm(out, state, want)
+
+
 # ----------------------------------------------------------------------------------------------------------- attention with sinks
 ATTENTION_CASES = [
     # contexts, query heads, KV heads, head size, block, window, sinks
@@ -437,6 +492,39 @@ def test_attention_with_sinks_over_quantized_pools_on_the_cpu(fmt):
     got = run_attention(a, ctx, Hq, Hkv, D, bs, 20, 3, "cpu").double()
     o, _ = attention_oracle(a[0], a[4], a[5], a[3], ctx, Hkv, bs, D ** -0.5, 20, 3)
     assert float((got - o).abs().max() / o.abs().max()) < 4 * 2.0 ** -8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,splits", [("bf16", s) for s in range(1, 9)] + [("fp8", 1), ("fp8", 3), ("int4", 5)])
+def test_every_split_gives_the_same(fmt, splits):
+    ctx, Hq, Hkv, D, bs = [700, 1, 333, 0], 16, 2, 128, 16
+    a = attention_inputs("cuda", ctx, Hq, Hkv, D, bs, fmt)
+    out = torch.full((4, Hq, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+    k, v = (a[1], a[2]) if fmt == "bf16" else (a[1].data, a[2].data)
+    ks, vs = (None, None) if fmt == "bf16" else (a[1].scale, a[2].scale)
+    torch.ops.mmb200.sink_decode(a[0], k, v, ks, vs, a[3].cuda(), torch.tensor(ctx, dtype=torch.int32, device="cuda"), out, Hq, Hkv, D, bs, D ** -0.5, 500, 20,
+                                 -1 if fmt == "bf16" else a[1].fmt_code, splits)
+    check_attention(out, attention_oracle(a[0], a[4], a[5], a[3], ctx, Hkv, bs, D ** -0.5, 500, 20))
+
+
+@pytest.mark.gpu
+def test_value_scales_that_grow_along_the_sequence():
+    """Rows of one cache differ by many powers of two: small rows in front, large ones behind, and the other way round."""
+    Hq, Hkv, D, bs, n = 8, 1, 128, 16, 200
+    for flip in (False, True):
+        rn = gen(5, "cuda")
+        mag = torch.logspace(-3, 3, n, device="cuda")[:, None, None]
+        mag = mag.flip(0) if flip else mag
+        pools, exact = [], []
+        for m in (torch.ones_like(mag), mag):
+            pool = ops.FP8KV(208, (Hkv, D), "cuda", "fp8")
+            pool.store(torch.arange(n, device="cuda"), rn(n, Hkv, D) * m)
+            pools.append(pool)
+            exact.append((pool._decode(pool.data).double() * pool.scale.double()[..., None]).cpu())
+        q = rn(1, Hq, D).to(torch.bfloat16)
+        tables = torch.arange(13, dtype=torch.int32)[None]
+        got = run_attention((q, pools[0], pools[1], tables), [n], Hq, Hkv, D, bs, 150, 8, "cuda")
+        check_attention(got, attention_oracle(q, exact[0], exact[1], tables, [n], Hkv, bs, D ** -0.5, 150, 8))
 
 
 @pytest.mark.gpu
@@ -487,6 +575,9 @@ def test_blocks_and_rows_outside_the_pools_are_hidden_and_reported():
     tables = a[3].clone()
     tables[0, 1] = 10 ** 6
     got = run_attention((*a[:3], tables), ctx, Hq, Hkv, D, bs, 40, 2, "cuda")
+    assert ops.check_status(dev) == 131
+    ops.clear_status(dev)
+    run_attention((*a[:3], a[3][:, :2].contiguous()), ctx, Hq, Hkv, D, bs, 40, 2, "cuda")            # 48 tokens, a table for 32
     assert ops.check_status(dev) == 131
     ops.clear_status(dev)
     pos = [p for p in range(48) if (p < 2 or p >= 8) and p // bs != 1]
