@@ -229,6 +229,7 @@ typedef struct {
   long long q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, o_tok_stride, o_head_stride;
   float scale;
   int window;             // 0 = none; > 0: query position x sees the keys (x - window, x]
+  int sinks;              // with a window: the keys 0 .. sinks - 1 stay visible too
   int* status;            // device int: 31..36 after a bounded wait expired (producer, mma, softmax stages)
 } MmbFmhaPrefillParams;
 int mmb_fmha_prefill(const MmbFmhaPrefillParams* p, cudaStream_t stream);

@@ -14,7 +14,7 @@
 //   S = Q K^T: the contraction may be permuted, so a lane reads 8 consecutive values (16 bytes of bf16) of its key and uses them as the B
 //   fragments of two k-steps; Q is held in the same order.
 //   O = P V: the output columns may be permuted, so a lane reads 8 consecutive columns of its four keys and pairs them up with byte permutes.
-// P is split into two 16-bit numbers (P = hi + lo to 2^-17): a single bf16 P would add as much error as rounding the output does.  Up to 8 heads
+// P is split into two 16-bit numbers (P = hi + lo to 2^-16): a single bf16 P would add as much error as rounding the output does.  Up to 8 heads
 // fill only half of the 16 rows; hi and lo then take rows 0-7 and 8-15 of ONE product.  9 to 16 heads take two products.
 //
 // Quantized pools: the codes of every format are exact in f16, so both products run in f16.  Q goes in divided by a power of two per row, undone in

@@ -1,6 +1,7 @@
 // torch.ops.mmb200.* : thin argument-checking shims over the extern "C" kernel launchers.
 // Every op writes into caller-provided output tensors (no allocation here), runs on the current
 // CUDA stream and is therefore capturable in a CUDA graph.
+#include <climits>
 #include <cstring>
 
 #include <ATen/cuda/CUDAContext.h>
@@ -1341,8 +1342,8 @@ void moe_combine(const Tensor& y, const Tensor& inv, const OptT& add0, const Opt
 
 // Causal prefill attention of one sequence on the tcgen05 path.  q [t, Hq, D], k [n, Hk, D] (last dim contiguous),
 // vt [Hk, D, n_pad] contiguous, out [t, Hq, D]; status: device int tensor (first word receives a code after a timeout).
-void fmha_prefill(const Tensor& q, const Tensor& k, const Tensor& vt, Tensor out, int64_t n, double scale, Tensor status,
-                  int64_t window) {
+void fmha_prefill_sinks(const Tensor& q, const Tensor& k, const Tensor& vt, Tensor out, int64_t n, double scale, Tensor status,
+                        int64_t window, int64_t sinks) {
   check_bf16(q, "q");
   check_bf16(k, "k");
   check_bf16(vt, "vt");
@@ -1371,9 +1372,14 @@ void fmha_prefill(const Tensor& q, const Tensor& k, const Tensor& vt, Tensor out
   p.o_tok_stride = out.stride(0);
   p.o_head_stride = out.stride(1);
   p.scale = (float)scale;
+  TORCH_CHECK_VALUE(window >= 0 && window <= INT_MAX && sinks >= 0 && sinks <= INT_MAX / 2, "window and sinks must not be negative");
   p.window = (int)window;
+  p.sinks = (int)sinks;
   p.status = status.data_ptr<int>();
   check(mmb_fmha_prefill(&p, cur_stream()), "fmha_prefill");
+}
+void fmha_prefill(const Tensor& q, const Tensor& k, const Tensor& vt, Tensor out, int64_t n, double scale, Tensor status, int64_t window) {
+  fmha_prefill_sinks(q, k, vt, out, n, scale, status, window, 0);
 }
 
 // In-switch all-reduce of the first `n` fp32 elements of a symmetric buffer.  desc (CPU int64 [6]): multicast address of the
@@ -1430,6 +1436,7 @@ Tensor vmm_tensor(int64_t id, int64_t nbytes, int64_t dev) {
 
 TORCH_LIBRARY(mmb200, m) {
   m.def("fmha_prefill", &fmha_prefill);
+  m.def("fmha_prefill_sinks", &fmha_prefill_sinks);
   m.def("fp4_gemm_grouped", &fp4_gemm_grouped);
   m.def("bf16_gemm", &bf16_gemm);
   m.def("fp4_gemv", &fp4_gemv);

@@ -321,34 +321,39 @@ class Transformer:
         out = torch.empty(q.shape[0], Hq * D, dtype=torch.bfloat16, device=q.device)
         bs = kv.block_size
         win = int(cfg.sliding_window or 0)
-        sinks = int(cfg.attention_sinks or 0) if win else 0      # the gathers below cut off everything in front of the window: not with sinks
+        sinks = int(cfg.attention_sinks or 0) if win else 0
 
         def _first_key(t, n_ctx):
             # with a sliding window only the keys the chunk's first query can still see are gathered
             return max(0, n_ctx - t - win + 1) if win else 0
 
         def _rows(pool, b, lo, n_ctx):
-            """bf16 rows ``[n_ctx - lo, Hk, D]`` of sequence ``b``'s cached keys or values (quantized pools are expanded by
-            their gather kernel, with the window's leading rows cut off afterwards)."""
+            """bf16 rows of sequence ``b``'s cached keys or values from position ``lo`` on, behind those of the sinks in front of it: leaving
+            out what nobody sees moves queries and window alike, so the mask stays right (quantized pools are expanded by their gather
+            kernel, and the rows picked afterwards)."""
+            keep = min(sinks, lo)
             if isinstance(pool, ops.FP8KV):
                 cu_k = meta.cached(("cu_k1", n_ctx), lambda: torch.tensor([0, n_ctx], dtype=torch.int32, device=q.device))
-                return ops.kv_fp8_rows(pool, meta.block_tables[b:b + 1], meta.ctx_lens[b:b + 1], cu_k, n_ctx, n_ctx, bs)[lo:]
+                rows = ops.kv_fp8_rows(pool, meta.block_tables[b:b + 1], meta.ctx_lens[b:b + 1], cu_k, n_ctx, n_ctx, bs)
+                return torch.cat([rows[:keep], rows[lo:]]) if 0 < keep < lo else rows[lo - keep:]
 
             def _slots():
                 tok = torch.arange(lo, n_ctx, device=q.device)
+                if keep:
+                    tok = torch.cat([torch.arange(keep, device=q.device), tok])
                 return meta.block_tables[b, tok // bs].long() * bs + tok % bs
             return pool.view(-1, Hk, D)[meta.cached(("slots", b, lo, n_ctx), _slots)]
 
-        if (not sinks and meta.attn_mask is None and q.dtype == torch.bfloat16 and len(meta.cu_seqlens) == 2 and q.stride(2) == 1
+        if (meta.attn_mask is None and q.dtype == torch.bfloat16 and len(meta.cu_seqlens) == 2 and q.stride(2) == 1
                 and ops.fmha_ok(q.shape[0], int(meta.ctx_lens_host[0]), D, D, q.device)):
             # one long sequence: its cache rows (this chunk included) gathered once, then the tcgen05 attention kernel
             n_ctx = int(meta.ctx_lens_host[0])
             lo = _first_key(q.shape[0], n_ctx)
             ops.fmha_prefill(q, _rows(kv.k[li], 0, lo, n_ctx), _rows(kv.v[li], 0, lo, n_ctx), out.view(-1, Hq, D), self.scale,
-                             window=win)
+                             window=win, sinks=sinks)
             return out
         n_seq = len(meta.cu_seqlens) - 1
-        if (not sinks and meta.attn_mask is None and q.dtype == torch.bfloat16 and n_seq > 1 and q.stride(2) == 1
+        if (meta.attn_mask is None and q.dtype == torch.bfloat16 and n_seq > 1 and q.stride(2) == 1
                 and all(ops.fmha_ok(meta.cu_seqlens[b + 1] - meta.cu_seqlens[b], int(meta.ctx_lens_host[b]), D, D, q.device)
                         for b in range(n_seq))):
             # several long sequences: the tcgen05 attention kernel sequence by sequence (a launch per sequence costs
@@ -358,7 +363,7 @@ class Transformer:
                 n_ctx = int(meta.ctx_lens_host[b])
                 lo = _first_key(e0 - s0, n_ctx)
                 ops.fmha_prefill(q[s0:e0], _rows(kv.k[li], b, lo, n_ctx), _rows(kv.v[li], b, lo, n_ctx),
-                                 out[s0:e0].view(-1, Hq, D), self.scale, window=win)
+                                 out[s0:e0].view(-1, Hq, D), self.scale, window=win, sinks=sinks)
             return out
         if meta.attn_mask is None and q.dtype == torch.bfloat16:
             # one launch for all sequences: keys are read from the paged pool through the block table

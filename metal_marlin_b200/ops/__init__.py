@@ -1214,10 +1214,10 @@ def fmha_ok(t: int, n: int, D: int, Dv: int, device) -> bool:
                 and torch.device(device).type == "cuda" and native_available() and not _FORCE_REF)
 
 
-def fmha_prefill(q, k, v, out, scale, vt=None, window=0):
+def fmha_prefill(q, k, v, out, scale, vt=None, window=0, sinks=0):
     """Causal attention of ONE sequence on the tcgen05 kernel (``csrc/attention_fmha_sm100.cu``): ``q [t, Hq, D]`` are the last
     ``t`` positions of the keys ``k, v [n, Hk, D]``; ``D`` 128 or 256.  With ``window > 0`` a query sees only the last
-    ``window`` keys up to its own position, and key tiles in front of a query tile's window are skipped.  The kernel takes V transposed per head, ``vt [Hk, D,
+    ``window`` keys up to its own position and the first ``sinks`` keys, and key tiles between the two are skipped.  The kernel takes V transposed per head, ``vt [Hk, D,
     n_pad]`` with ``n_pad % 8 == 0`` and zeros behind column ``n`` (the B operand of its P V MMA is K-major like every other
     operand); callers that can produce it directly (a GEMM with swapped operands) pass ``vt``, else it is built here with
     one strided copy of ``v``."""
@@ -1229,7 +1229,10 @@ def fmha_prefill(q, k, v, out, scale, vt=None, window=0):
         vt[:, :, :n].copy_(v.permute(1, 2, 0))
         if n_pad > n:
             vt[:, :, n:].zero_()
-    K.mmb200.fmha_prefill(q, k, vt, out, n, float(scale), gemm_status(q.device), int(window or 0))
+    if sinks:
+        K.mmb200.fmha_prefill_sinks(q, k, vt, out, n, float(scale), gemm_status(q.device), int(window or 0), int(sinks))
+    else:
+        K.mmb200.fmha_prefill(q, k, vt, out, n, float(scale), gemm_status(q.device), int(window or 0))
     return out
 
 

@@ -129,7 +129,7 @@ def attention_oracle(q, k, v, tables, ctx, Hkv, bs, scale, window, sinks, kf=Non
         o = torch.einsum("hgt,thd->hgd", pr, vv)
         w = torch.einsum("hgt,thd->hgd", pr, vv.abs())
         # scores: D fp32 products summed (2^-23 a step) and a few roundings of scale; exponentials 2^-21 and their argument; P in two bf16
-        # parts 2^-17; sums over the keys 2^-23 a key; numerator and denominator alike
+        # parts 2^-16; sums over the keys 2^-23 a key; numerator and denominator alike
         rel = m.amax(-1) * (D + 8) * 2.0 ** -23 + s.abs().amax(-1) * 2.0 ** -22 + 2.0 ** -16 + len(pos) * 2.0 ** -23
         out[b], err[b] = o.reshape(Hq, D), (2 * rel[..., None] * w).reshape(Hq, D)
     return out, err

@@ -83,3 +83,57 @@ def test_engine_serves_windowed_streams(preset, kv_dtype):
     assert [g[0] for g in got] == [w[0] for w in alone]
     assert same >= 12                                     # 15 tokens; a near tie may fall otherwise at another batch size
     assert ops.check_status(torch.device("cuda")) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t,n,Hq,Hk,D,window,sinks", [(1024, 1024, 4, 2, 128, 64, 4), (700, 1536, 4, 2, 128, 300, 129), (300, 900, 2, 2, 256, 100, 65),
+                                                      (512, 2048, 2, 1, 256, 1000, 1), (640, 640, 2, 2, 128, 4096, 7), (384, 1200, 4, 4, 128, 1, 200),
+                                                      (257, 700, 2, 1, 128, 250, 5000), (256, 256, 1, 1, 128, 129, 128)])
+def test_prompt_attention_with_sinks_on_the_tensor_cores(t, n, Hq, Hk, D, window, sinks):
+    """Tiles of the sinks, a gap, then the window's tiles.  What a kernel may round: P and the output to bf16, which keeps 8 significant bits, so
+    half a step is finfo.eps / 2 = 2^-8 of the value (of sum p |v| and of the output); scores in fp32."""
+    g = torch.Generator().manual_seed(t + n)
+    q, k, v = (torch.randn(m, h, D, generator=g).to(torch.bfloat16).cuda() for m, h in ((t, Hq), (n, Hk), (n, Hk)))
+    out = torch.empty(t, Hq, D, dtype=torch.bfloat16, device="cuda")
+    ops.fmha_prefill(q, k, v, out, D ** -0.5, window=window, sinks=sinks)
+    assert ops.check_status(torch.device("cuda")) == 0
+    qd, kd, vd = q.double(), k.double().repeat_interleave(Hq // Hk, 1), v.double().repeat_interleave(Hq // Hk, 1)
+    s = torch.einsum("thd,nhd->htn", qd, kd) * D ** -0.5
+    m = torch.einsum("thd,nhd->htn", qd.abs(), kd.abs()).amax(-1) * D ** -0.5
+    pos, key = torch.arange(n - t, n, device="cuda")[:, None], torch.arange(n, device="cuda")
+    p = torch.softmax(s.masked_fill(~((key <= pos) & ((key > pos - window) | (key < sinks))), float("-inf")), -1)
+    o, w = torch.einsum("htn,nhd->thd", p, vd), torch.einsum("htn,nhd->thd", p, vd.abs())
+    rel = (2 * ((D + 8) * 2.0 ** -23 * m + n * 2.0 ** -23 + 2.0 ** -18)).t()[..., None]
+    half = 1.01 * torch.finfo(torch.bfloat16).eps / 2
+    gap = (out.double() - o).abs() - ((half + rel) * w + half * (o.abs() + (half + rel) * w))
+    assert (gap <= 0).all(), float(gap.max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_dtype", ["bf16", "int8"])
+def test_long_prompts_of_a_windowed_model(kv_dtype):
+    """Chunked prompts far past the window, several sequences: the gathered sinks and window rows against the reference path."""
+    cfg = windowed("tiny-llama", 100, 6)
+    cfg.head_dim, cfg.num_attention_heads, cfg.num_key_value_heads = 128, 4, 2
+    lm = MMFP4ForCausalLM.from_config(cfg, device="cuda", seed=2)
+    g = torch.Generator().manual_seed(0)
+    prompts = [torch.randint(0, 1024, (n,), generator=g).tolist() for n in (900, 640)]
+    bt = torch.arange(2 * 60, dtype=torch.int32).view(2, 60)
+    calls, real = [], ops.fmha_prefill
+
+    def counting(*a, **kw):
+        calls.append((a[1].shape[0], kw.get("sinks")))
+        return real(*a, **kw)
+    ops.fmha_prefill = counting
+    try:
+        a = prefill(lm.model, lm.new_cache(120, 16, kv_dtype), prompts, bt, chunk_tokens=300)
+        b = prefill(lm.model, lm.new_cache(120, 16, kv_dtype), prompts, bt)
+    finally:
+        ops.fmha_prefill = real
+    assert calls and all(s == 6 for _, s in calls)
+    assert min(n for n, _ in calls) < 600                  # only sinks, window and chunk are gathered, not the whole context
+    with ops.force_reference():
+        c = prefill(lm.model, lm.new_cache(120, 16, kv_dtype), prompts, bt)
+    for x in (a, b):
+        assert float((x - c).abs().max() / c.abs().max()) < 6e-2
+    assert ops.check_status(torch.device("cuda")) == 0
