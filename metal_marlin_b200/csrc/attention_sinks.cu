@@ -10,21 +10,23 @@
 // distributed shared memory in the same launch.  No global workspace: captured graphs share nothing and no result depends on arrival order.
 // The reference of a row moves only when a score exceeds it by more than 2^8 (one vote for all rows; the usual tile has no shuffles).
 //
-// Tensor cores (m16n8k16): all query heads of a KV head are the rows of one product, so a key is read once.
-//   S = Q K^T: the contraction may be permuted, so a lane reads 8 consecutive values (16 bytes of bf16) of its key and uses them as the B
+// Tensor cores (m16n8k16): eight query heads of a KV head are the columns of a product (9 to 16 heads: of two), so a key is read once.
+//   S^T = K Q^T: the contraction may be permuted, so a lane reads 8 consecutive values (16 bytes of bf16) of a key and uses them as the A
 //   fragments of two k-steps; Q is held in the same order.
-//   O = P V: the output columns may be permuted, so a lane reads 8 consecutive columns of its four keys and pairs them up with byte permutes.
-// P is split into two 16-bit numbers (P = hi + lo to 2^-16): a single bf16 P would add as much error as rounding the output does.  Up to 8 heads
-// fill only half of the 16 rows; hi and lo then take rows 0-7 and 8-15 of ONE product.  9 to 16 heads take two products.
+//   O^T = V^T P^T: the output rows may be permuted, so a lane reads 8 consecutive columns of its four keys and pairs them up with byte permutes; P
+//   is transposed inside the warp (movmatrix).
+// With the heads as columns every accumulator belongs to a head; as rows (16 of them) up to 8 heads left half of the accumulators empty and took
+// twice the products for S (fp8, 64 rows: 143 us against 135; 8-bit cache of 256-wide heads 75 against 69).
+// P is split into two 16-bit numbers (P = hi + lo to 2^-16): a single bf16 P would add as much error as rounding the output does.
 //
 // Quantized pools: the codes of every format are exact in f16, so both products run in f16.  Q goes in divided by a power of two per row, undone in
 // the score; the row scale of K multiplies the score and that of V the probability, both in fp32.  Probabilities times value scales are kept in f16's
 // range by a reference for the scales (4 x the largest seen) and a factor of 2^7.
 //
-// Measured (graph replays, heads 32 / 8 of 128, window 4096 + 4, three input sets in turn): 64 rows bf16 164 us = 6.5 TB/s, the measured copy rate;
-// 8 rows 26 us; 1 row 11.5 us.  int8 32 rows 64 us and fp8 64 rows 141 us, 1.5 to 1.7 x the time of their bytes: half the bytes a key, the
+// Measured (graph replays, heads 32 / 8 of 128, window 4096 + 4, three input sets in turn): 64 rows bf16 166 us = 6.5 TB/s, the measured copy rate;
+// 8 rows 28 us; 1 row 11.8 us.  int8 32 rows 62 us and fp8 64 rows 135 us, 1.5 to 1.6 x the time of their bytes: half the bytes a key, the
 // same instructions a key plus the conversions, so the issue slots bound them (hardware conversions into f16 instead of bf16: int8 117 -> 76 us;
-// 32 keys a tile 76 -> 64).
+// 32 keys a tile 76 -> 64; rows padded instead of swizzled changed nothing, 62 -> 63).
 #include <atomic>
 #include <cuda_fp4.h>
 
@@ -124,6 +126,12 @@ __device__ __forceinline__ void sd_load8(const unsigned char* p, uint32_t (&w)[4
   } else {
     sd_load8_f16<F>(p, w);
   }
+}
+// 8 x 8 matrix of 16-bit values, two of a row in each lane, transposed.
+__device__ __forceinline__ uint32_t sd_transpose(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
 }
 template <int N>
 __device__ __forceinline__ float sd_max(const float (&v)[N]) {
@@ -255,22 +263,30 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
     sd_commit();
   };
 
+  constexpr int HT = R / 8;                                      // tiles of eight heads
   constexpr bool kQReg = D <= 128;
-  uint4 qr[kQReg ? NI : 1][WIDE ? 2 : 1];
+  uint4 qr[kQReg ? NI : 1][HT];
   if constexpr (kQReg) {
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int h = 0; h < (WIDE ? 2 : 1); ++h) qr[i][h] = *reinterpret_cast<const uint4*>(q_sm + ((gid + 8 * h) * (D / 8) + ((tig + 4 * i) ^ ((gid & 1) << 2))) * 16);
+      for (int h = 0; h < HT; ++h) qr[i][h] = *reinterpret_cast<const uint4*>(q_sm + ((gid + 8 * h) * (D / 8) + ((tig + 4 * i) ^ ((gid & 1) << 2))) * 16);
   }
-  float o[NJ * 8][4];
+  float o[NJ * 4][HT][4];
 #pragma unroll
-  for (int i = 0; i < NJ * 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int i = 0; i < NJ * 4; ++i)
+#pragma unroll
+    for (int h = 0; h < HT; ++h) o[i][h][0] = o[i][h][1] = o[i][h][2] = o[i][h][3] = 0.f;
   float v_ref = 0.f;                                             // quantized: reference of the value scales
-  float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};      // rows gid and (WIDE) gid + 8
-  const float c = p.scale * 1.4426950408889634f;
-  float cr[2] = {c, c};
-  if constexpr (kScaled) cr[0] = c * q_scale[gid], cr[1] = WIDE ? c * q_scale[gid + 8 * WIDE] : 0.f;
+  // this lane's heads: 8 h + 2 tig, + 1
+  float mx[2 * HT], l[2 * HT], cr[2 * HT];
+#pragma unroll
+  for (int h = 0; h < 2 * HT; ++h) {
+    mx[h] = -INFINITY;
+    l[h] = 0.f;
+    cr[h] = p.scale * 1.4426950408889634f;
+    if constexpr (kScaled) cr[h] *= q_scale[8 * (h >> 1) + 2 * tig + (h & 1)];
+  }
 
 #pragma unroll
   for (int t = 0; t < NST - 1; ++t) issue(t, slot_of(t));
@@ -283,114 +299,118 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
     const unsigned char* st = ring + (t % NST) * Cfg::stage_bytes;
     const unsigned char* vt = st + Cfg::tile_bytes / 2;
     const unsigned ok = ok_sm[warp][t % NST];
-    float s[NT][4] = {}, s2[NT][4] = {};
+    // S^T = K Q^T, two chains a tile
+    float s[KT][HT][4] = {}, s2[KT][HT][4] = {};
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int pc = tig + 4 * i;
-      uint4 qa, qb = make_uint4(0, 0, 0, 0);
-      if constexpr (kQReg) {
-        qa = qr[i][0];
-        if constexpr (WIDE) qb = qr[i][WIDE];
-      } else {
-        qa = *reinterpret_cast<const uint4*>(q_sm + (gid * (D / 8) + (pc ^ ((gid & 1) << 2))) * 16);
-        if constexpr (WIDE) qb = *reinterpret_cast<const uint4*>(q_sm + ((gid + 8) * (D / 8) + (pc ^ ((gid & 1) << 2))) * 16);
+      uint4 q[HT];
+#pragma unroll
+      for (int h = 0; h < HT; ++h) {
+        if constexpr (kQReg) q[h] = qr[i][h];
+        else q[h] = *reinterpret_cast<const uint4*>(q_sm + ((gid + 8 * h) * (D / 8) + (pc ^ ((gid & 1) << 2))) * 16);
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int r = gid + 8 * nt;
-        uint32_t w[4];
-        const unsigned char* kp = st + (r * U + sd_unit_k<U, Cfg::piece>(r, pc * Cfg::piece / 16)) * 16 + pc * Cfg::piece % 16;
-        sd_load8<F>(kp, w);
-        sd_mma<F>(s[nt], qa.x, qb.x, qa.y, qb.y, w[0], w[1]);
-        sd_mma<F>(s2[nt], qa.z, qb.z, qa.w, qb.w, w[2], w[3]);
+      for (int kt = 0; kt < KT; ++kt) {
+        uint32_t w[2][4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = 16 * kt + 8 * e + gid;
+          sd_load8<F>(st + (r * U + sd_unit_k<U, Cfg::piece>(r, pc * Cfg::piece / 16)) * 16 + pc * Cfg::piece % 16, w[e]);
+        }
+#pragma unroll
+        for (int h = 0; h < HT; ++h) {
+          sd_mma<F>(s[kt][h], w[0][0], w[1][0], w[0][1], w[1][1], q[h].x, q[h].y);
+          sd_mma<F>(s2[kt][h], w[0][2], w[1][2], w[0][3], w[1][3], q[h].z, q[h].w);
+        }
       }
     }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < (WIDE ? 4 : 2); ++e) s[nt][e] += s2[nt][e];
-    // scores in units of log2; this lane's keys are 8 nt + 2 tig, + 1
-    float p4[2][2 * NT];                                         // [row half][key]
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int key = 8 * nt + 2 * tig + e;
-        float f = 1.f;
-        if constexpr (kScaled) f = reinterpret_cast<const float*>(st + Cfg::tile_bytes)[key];
-        const bool in = ok >> key & 1;
-        p4[0][2 * nt + e] = in ? s[nt][e] * (cr[0] * f) : -INFINITY;
-        p4[1][2 * nt + e] = in ? s[nt][2 + e] * (cr[1] * f) : -INFINITY;
-      }
-    // the reference of a row moves only when one of its scores is more than kSdLazy above it; the test is one vote for all rows
+    // scores in units of log2; this lane's keys are 8 k + gid
+    float p4[2 * HT][NT];                                        // [head][key]
     bool grew = false;
-    float vs[2 * NT] = {};
-    if constexpr (kScaled) {
+    float vs[NT] = {};
 #pragma unroll
-      for (int k = 0; k < 2 * NT; ++k) {
-        vs[k] = reinterpret_cast<const float*>(st + Cfg::tile_bytes)[T + 8 * (k >> 1) + 2 * tig + (k & 1)];
+    for (int k = 0; k < NT; ++k) {
+      const int key = 8 * k + gid;
+      float f = 1.f;
+      if constexpr (kScaled) {
+        f = reinterpret_cast<const float*>(st + Cfg::tile_bytes)[key];
+        vs[k] = reinterpret_cast<const float*>(st + Cfg::tile_bytes)[T + key];
         grew |= vs[k] > v_ref;
       }
-    }
+      const bool in = ok >> key & 1;
 #pragma unroll
-    for (int h = 0; h < (WIDE ? 2 : 1); ++h) grew |= sd_max(p4[h]) > mx[h] + kSdLazy;
+      for (int h = 0; h < 2 * HT; ++h) {
+        const int c = 2 * (k & 1) + (h & 1);
+        p4[h][k] = in ? (s[k >> 1][h >> 1][c] + s2[k >> 1][h >> 1][c]) * (cr[h] * f) : -INFINITY;
+      }
+    }
+    // the reference of a head moves only when one of its scores is more than kSdLazy above it; the test is one vote for all heads
+#pragma unroll
+    for (int h = 0; h < 2 * HT; ++h) grew |= sd_max(p4[h]) > mx[h] + kSdLazy;
     if (__any_sync(0xffffffffu, grew)) {
-      float alpha[2] = {1.f, 1.f}, beta = 1.f;
+      float alpha[2 * HT], beta = 1.f;
+      auto lanes_max = [](float m) {                             // over the lanes that hold other keys of the same heads
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        return m;
+      };
       if constexpr (kScaled) {
-        float m = sd_max(vs);
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const float m = lanes_max(sd_max(vs));
         if (m > v_ref) {
           beta = v_ref / (4.f * m);
           v_ref = 4.f * m;
         }
       }
 #pragma unroll
-      for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
-        float t4 = sd_max(p4[h]);
-        t4 = fmaxf(t4, __shfl_xor_sync(0xffffffffu, t4, 1));
-        t4 = fmaxf(t4, __shfl_xor_sync(0xffffffffu, t4, 2));
-        if (t4 > mx[h]) {
-          alpha[h] = sd_exp2(mx[h] - t4);
-          mx[h] = t4;
-          l[h] *= alpha[h];
+      for (int h = 0; h < 2 * HT; ++h) {
+        const float m = lanes_max(sd_max(p4[h]));
+        alpha[h] = beta;
+        if (m > mx[h]) {
+          const float f = sd_exp2(mx[h] - m);
+          mx[h] = m;
+          l[h] *= f;
+          alpha[h] *= f;
         }
       }
-      const float a0 = alpha[0] * beta, a1 = (WIDE ? alpha[1] : alpha[0]) * beta;
 #pragma unroll
-      for (int i = 0; i < NJ * 8; ++i) o[i][0] *= a0, o[i][1] *= a0, o[i][2] *= a1, o[i][3] *= a1;
+      for (int i = 0; i < NJ * 4; ++i)
+#pragma unroll
+        for (int h = 0; h < HT; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][h][e] *= alpha[2 * h + (e & 1)];
     }
+    const float inv = kScaled && v_ref > 0.f ? 128.f / v_ref : 0.f;
 #pragma unroll
-    for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
+    for (int h = 0; h < 2 * HT; ++h) {
       const float ref = mx[h] == -INFINITY ? 0.f : mx[h];
 #pragma unroll
-      for (int k = 0; k < 2 * NT; ++k) p4[h][k] = sd_exp2(p4[h][k] - ref);
-#pragma unroll
-      for (int k = 0; k < 2 * NT; k += 4) l[h] += (p4[h][k] + p4[h][k + 1]) + (p4[h][k + 2] + p4[h][k + 3]);
-    }
-    if constexpr (kScaled) {
-      const float inv = v_ref > 0.f ? 128.f / v_ref : 0.f;
-#pragma unroll
-      for (int k = 0; k < 2 * NT; ++k) {
-        p4[0][k] *= vs[k] * inv;
-        if constexpr (WIDE) p4[1][k] *= vs[k] * inv;
+      for (int k = 0; k < NT; ++k) {
+        p4[h][k] = sd_exp2(p4[h][k] - ref);
+        l[h] += p4[h][k];
+        if constexpr (kScaled) p4[h][k] *= vs[k] * inv;
       }
     }
-    uint32_t hi[2][NT], lw[2][NT];                               // [row half][eight keys]
+    // P as B fragments: [8 keys][8 heads] of this layout, transposed inside the warp
+    uint32_t hi[HT][NT], lw[HT][NT];
 #pragma unroll
-    for (int h = 0; h < (WIDE ? 2 : 1); ++h)
+    for (int h = 0; h < HT; ++h)
 #pragma unroll
       for (int k = 0; k < NT; ++k) {
-        const float x = p4[h][2 * k], y = p4[h][2 * k + 1];
+        const float x = p4[2 * h][k], y = p4[2 * h + 1][k];
+        uint32_t a, b;
         if constexpr (kScaled) {
-          hi[h][k] = pack16(x, y, 1);
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[h][k]));
-          lw[h][k] = pack16(x - f.x, y - f.y, 1);
+          a = pack16(x, y, 1);
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+          b = pack16(x - f.x, y - f.y, 1);
         } else {
-          hi[h][k] = sd_pack(x, y);
-          lw[h][k] = sd_pack(x - __uint_as_float(hi[h][k] << 16), y - __uint_as_float(hi[h][k] & 0xffff0000u));
+          a = sd_pack(x, y);
+          b = sd_pack(x - __uint_as_float(a << 16), y - __uint_as_float(a & 0xffff0000u));
         }
+        hi[h][k] = sd_transpose(a);
+        lw[h][k] = sd_transpose(b);
       }
+    // O^T += V^T P^T
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -403,50 +423,44 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
           sd_load8<F>(vt + (r * U + sd_unit_v<U, Cfg::piece>(r, pc * Cfg::piece / 16)) * 16 + pc * Cfg::piece % 16, v[k]);
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t sel = e & 1 ? 0x7632u : 0x5410u;
-          const uint32_t b0 = __byte_perm(v[0][e >> 1], v[1][e >> 1], sel), b1 = __byte_perm(v[2][e >> 1], v[3][e >> 1], sel);
-          if constexpr (WIDE) {
-            sd_mma<F>(o[jj * 8 + e], hi[0][2 * kt], hi[1][2 * kt], hi[0][2 * kt + 1], hi[1][2 * kt + 1], b0, b1);
-            sd_mma<F>(o[jj * 8 + e], lw[0][2 * kt], lw[1][2 * kt], lw[0][2 * kt + 1], lw[1][2 * kt + 1], b0, b1);
-          } else {
-            sd_mma<F>(o[jj * 8 + e], hi[0][2 * kt], lw[0][2 * kt], hi[0][2 * kt + 1], lw[0][2 * kt + 1], b0, b1);
+        for (int m = 0; m < 4; ++m) {                            // rows gid: column 2 m of the piece, rows gid + 8: column 2 m + 1
+          const uint32_t a0 = __byte_perm(v[0][m], v[1][m], 0x5410), a1 = __byte_perm(v[0][m], v[1][m], 0x7632);
+          const uint32_t a2 = __byte_perm(v[2][m], v[3][m], 0x5410), a3 = __byte_perm(v[2][m], v[3][m], 0x7632);
+#pragma unroll
+          for (int h = 0; h < HT; ++h) {
+            sd_mma<F>(o[jj * 4 + m][h], a0, a1, a2, a3, hi[h][2 * kt], hi[h][2 * kt + 1]);
+            sd_mma<F>(o[jj * 4 + m][h], a0, a1, a2, a3, lw[h][2 * kt], lw[h][2 * kt + 1]);
           }
         }
       }
     __syncwarp();                                                // the stage may be refilled
   }
 
-  // ---- join the warps.  Row r of warp w: maximum and sum in ml, O in the (idle) ring as [w][r][D]
+  // ---- join the warps.  Head r of warp w: maximum and sum in ml, O in the (idle) ring as [w][r][D]
   sd_wait<0>();
   __syncthreads();
 #pragma unroll
-  for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    if (tig == 0) ml[warp][gid + 8 * h][0] = mx[h], ml[warp][gid + 8 * h][1] = l[h];
+  for (int h = 0; h < 2 * HT; ++h) {
+#pragma unroll
+    for (int d = 4; d < 32; d *= 2) l[h] += __shfl_xor_sync(0xffffffffu, l[h], d);
+    if (gid == 0) ml[warp][8 * (h >> 1) + 2 * tig + (h & 1)][0] = mx[h], ml[warp][8 * (h >> 1) + 2 * tig + (h & 1)][1] = l[h];
   }
   float* os = reinterpret_cast<float*>(sm);
+  const float back = kScaled ? v_ref * (1.f / 128.f) : 1.f;
 #pragma unroll
   for (int jj = 0; jj < NJ; ++jj)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {                                // columns (2 tig + e + 8 jj) 8 .. + 7
-      const int col = (2 * tig + e + 8 * jj) * 8;
+    for (int h = 0; h < HT; ++h)
 #pragma unroll
-      for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
-        float4* dst = reinterpret_cast<float4*>(os + ((warp * R + gid + 8 * h) * D + col));
+      for (int e = 0; e < 2; ++e) {                              // head 8 h + 2 tig + e, columns 8 (gid + 8 jj) .. + 7
+        float4* dst = reinterpret_cast<float4*>(os + ((warp * R + 8 * h + 2 * tig + e) * D + (gid + 8 * jj) * 8));
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          float f[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float (&x)[4] = o[jj * 8 + q * 4 + i];
-            f[i] = (WIDE ? x[2 * h + e] : x[e] + x[2 + e]) * (kScaled ? v_ref * (1.f / 128.f) : 1.f);
-          }
-          dst[q] = make_float4(f[0], f[1], f[2], f[3]);
+          const float(&x)[4] = o[jj * 4 + 2 * q][h];
+          const float(&y)[4] = o[jj * 4 + 2 * q + 1][h];
+          dst[q] = make_float4(x[e] * back, x[2 + e] * back, y[e] * back, y[2 + e] * back);
         }
       }
-    }
   __syncthreads();
   // weights of the warps of row r: 2^(m_w - M)
   auto weight = [](float mw, float M) { return mw == -INFINITY ? 0.f : sd_exp2(mw - M); };
@@ -535,8 +549,8 @@ static int launch_sinks(const MmbSinkDecodeParams& p, cudaStream_t stream) {
   if (splits == 0) {
     const long long most = min((long long)p.window + p.sinks, (long long)p.max_blocks * p.block_size);
     const long long tiles = (most + Cfg::T - 1) / Cfg::T, rows = (long long)p.B * p.Hkv * hg;
-    // as many as the SMs hold at once: a second wave costs more than idle slots (24 rows of 8 KV heads: 1 split 74 us, 3 splits 87), a larger cluster
-    // more than it saves once the SMs are full (64 rows: 1 split 164 us, 2 splits 177, 8 splits 232)
+    // as many as the SMs hold at once: a second wave costs more than idle slots (24 rows of 8 KV heads: 1 split 73 us, 3 splits 88), a larger cluster
+    // more than it saves once the SMs are full (64 rows: 1 split 166 us, 2 splits 180, 8 splits 236)
     splits = 1;
     while (splits < 8 && rows * (splits + 1) <= 148 * ctas && (splits + 1) * kSdWarps <= tiles) ++splits;
   }
