@@ -9,11 +9,15 @@
 // per sequence, not over the flat token axis: with TT >= K - 1 only a sequence's first tile reads its old window, and the same thread writes the
 // new one (from x, or from the old window where the sequence is shorter than it), so the window is updated in place without a second launch.
 // Tile i belongs to the sequence s with base(s) <= i < base(s + 1), base(s) = cu[s] / TT + s: at least ceil(len / TT) tiles a sequence, found by
-// bisection, nothing counted on the host.  Measured, 8111 rows of 10240 channels, 4 taps, bf16: 72 us = 4.6 TB/s; two special functions a value
-// take 37 us of it, the bytes 51 us (conversions between the loads of a batch: 332 us; a choice by type at every value: 93 us).
+// bisection, nothing counted on the host.  Measured, 8111 rows of 10240 channels, 4 taps, bf16: 71 us = 4.7 TB/s (the bytes 51 us, two special
+// functions a value 37).  Without the activation it takes 66 us, with 24 instead of 16 warps an SM or 16-byte instead of 8-byte loads the same: bound by
+// the waves' starts and by reading and writing at once, not by arithmetic.  What it took: conversions between the loads of a batch 332 us; a choice by
+// type at every value 93; arithmetic on one value instead of two an instruction 75.
 //
 // Single tokens.  A thread owns V channels of RB rows: the taps are read once for RB rows, the window (V (K - 1) consecutive floats) moves
-// through registers.  256 rows of 10240 channels: 14.6 us = 5.0 TB/s.
+// through registers.  256 rows of 10240 channels: 14.6 us = 5.0 TB/s; 4096 channels of 8 taps, fp32: 16.4 us (windows moved by single floats: 55 us).
+#include <atomic>
+
 #include "api_ext.h"
 #include "launch.h"
 #include "typed_io.cuh"
@@ -23,29 +27,90 @@ namespace mmb {
 constexpr int kConvThreads = 128;
 constexpr int kConvSeqs = 1024;              // starts of this many sequences are kept in shared memory
 
-__device__ __forceinline__ float conv_act(float y, int act) { return act == 1 ? silu(y) : y; }
-
-// Taps and bias of V channels; taps that are compiled in but not used are zero.  The V K values of 16-bit weights lie together: whole words.
-template <int KT, int V>
-__device__ __forceinline__ void load_taps(const MmbCausalConvParams& p, int c0, int K, float (&w)[KT][V], float (&b)[V]) {
-  const int skip = KT - K;
-  const long long at = (long long)c0 * K;
-  if (KT < 8 && KT * V % 8 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0) {
-    float f[KT * V];
+// a = w x + a for V channels.
+template <int V>
+__device__ __forceinline__ void fma_v(float (&a)[V], const float (&w)[V], const float (&x)[V]) {
+  if constexpr (V % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < KT * V / 8; ++i) ldv<8>(p.w, at + 8 * i, p.wt, f + 8 * i);
+    for (int v = 0; v < V; v += 2) {
+      const float2 f = unpack2(fma2(pack2(w[v], w[v + 1]), pack2(x[v], x[v + 1]), pack2(a[v], a[v + 1])));
+      a[v] = f.x, a[v + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) a[v] = fmaf(w[v], x[v], a[v]);
+  }
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// x / (1 + e^-x)
+template <int V>
+__device__ __forceinline__ void silu_v(float (&x)[V]) {
+  constexpr float c = -1.4426950408889634f;
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int v = 0; v < V; v += 2) {
+      const f32x2 xx = pack2(x[v], x[v + 1]);
+      float2 f = unpack2(mul2(xx, pack2(c, c)));
+      f = unpack2(add2(pack2(exp2_fast(f.x), exp2_fast(f.y)), pack2(1.f, 1.f)));
+      f = unpack2(mul2(xx, pack2(rcp_fast(f.x), rcp_fast(f.y))));
+      x[v] = f.x, x[v + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] *= rcp_fast(1.f + exp2_fast(c * x[v]));
+  }
+}
+
+// Taps and bias of V channels.  The V K values of 16-bit weights lie together: whole words.
+template <int K, int V>
+__device__ __forceinline__ void load_taps(const MmbCausalConvParams& p, int c0, float (&w)[K][V], float (&b)[V]) {
+  constexpr int P = K * V % 8 == 0 ? 8 : 4;                // values a load
+  const long long at = (long long)c0 * K;
+  if (V == 4 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0) {
+    float f[K * V];
+#pragma unroll
+    for (int i = 0; i < K * V / P; ++i) ldv<P>(p.w, at + P * i, p.wt, f + P * i);
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
-      for (int k = 0; k < KT; ++k) w[k][v] = f[v * KT + k];
+      for (int k = 0; k < K; ++k) w[k][v] = f[v * K + k];
   } else {
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
-      for (int k = 0; k < KT; ++k) w[k][v] = k >= skip ? ld1(p.w, at + v * K + k - skip, p.wt) : 0.f;
+      for (int k = 0; k < K; ++k) w[k][v] = ld1(p.w, at + v * K + k, p.wt);
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) b[v] = p.bias ? ld1(p.bias, c0 + v, p.wt) : 0.f;
+}
+
+// The window of V channels: V W consecutive floats, in 16-byte pieces where it is aligned for that.
+template <int W, int V>
+__device__ __forceinline__ void ld_window(const float* st, bool vec, float (&win)[V * W]) {
+  if (V == 4 && vec) {
+#pragma unroll
+    for (int j = 0; j < V * W / 4; ++j) {
+      const float4 f = reinterpret_cast<const float4*>(st)[j];
+      win[4 * j] = f.x, win[4 * j + 1] = f.y, win[4 * j + 2] = f.z, win[4 * j + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V * W; ++j) win[j] = st[j];
+  }
+}
+template <int W, int V>
+__device__ __forceinline__ void st_window(float* st, bool vec, const float (&win)[V * W]) {
+  if (V == 4 && vec) {
+#pragma unroll
+    for (int j = 0; j < V * W / 4; ++j) reinterpret_cast<float4*>(st)[j] = make_float4(win[4 * j], win[4 * j + 1], win[4 * j + 2], win[4 * j + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V * W; ++j) st[j] = win[j];
+  }
 }
 
 template <int U, int V, int ES>
@@ -75,12 +140,10 @@ __device__ __forceinline__ void store_batch(void* out, long long at, long long l
   }
 }
 
-// KT taps are compiled in; `K` of them are used (K < KT only for KT = 8), aligned to the newest input: tap KT - 1 meets the newest one.
-template <int KT, int V, int ES>
-__global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCausalConvParams p, int n_groups, int TT, long long n_tiles) {
+template <int K, int V, int ES>
+__global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCausalConvParams p, int n_groups, int TT, long long n_tiles, bool vec_state) {
   constexpr int U = V == 4 && ES == 4 ? 4 : 8;             // tokens loaded together
-  constexpr int W = KT - 1;
-  const int K = KT == 8 ? p.K : KT, skip = KT - K;
+  constexpr int W = K - 1;
   pdl_launch_dependents();
   pdl_wait();
   // sequence starts in shared memory: the bisection would otherwise wait for global memory at every step
@@ -91,8 +154,8 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCaus
   const long long id = (long long)blockIdx.x * kConvThreads + threadIdx.x;
   const long long tile = id / n_groups;
   const int c0 = (int)(id - tile * n_groups) * V;
-  float w[KT][V], b[V], win[W][V];
-  if (tile < n_tiles) load_taps<KT, V>(p, c0, K, w, b);
+  float w[K][V], b[V], win[W][V];
+  if (tile < n_tiles) load_taps<K, V>(p, c0, w, b);
   __syncthreads();
   if (tile >= n_tiles) return;
   auto start = [&](int s) { return near ? starts[s] : min(max(p.cu_seqlens[s], 0), p.T); };
@@ -117,7 +180,7 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCaus
   if (first > 0) {
 #pragma unroll
     for (int j = 0; j < W; ++j)
-      if (j >= skip) ld_raw<V, ES>(p.x, (long long)(t0 - W + j) * p.ldx + c0, wr[j]);
+      ld_raw<V, ES>(p.x, (long long)(t0 - W + j) * p.ldx + c0, wr[j]);
   }
   long long row = -1;
   bool live = s < p.S;
@@ -134,38 +197,44 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCaus
   }
   if (first == 0) {
     const bool old = p.state && !(p.fresh && p.fresh[s]);
-    float* st = p.state ? p.state + (row * p.C + c0) * (K - 1) - skip : nullptr;
+    float* st = p.state ? p.state + (row * p.C + c0) * W : nullptr;
+    float was[V * W];
+    if (old) {
+      ld_window<W, V>(st, vec_state, was);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V * W; ++i) was[i] = 0.f;
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
-      for (int j = 0; j < W; ++j) win[j][v] = old && j >= skip ? st[v * (K - 1) + j] : 0.f;
+      for (int j = 0; j < W; ++j) win[j][v] = was[v * W + j];
     if (st) {
       const int len = end - begin;
+      Raw<V, ES> tail[W];                            // element j of the new window is input len - W + j; in front of the sequence, element j + len of the old
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        if (len - W + j >= 0) ld_raw<V, ES>(p.x, (long long)(end - W + j) * p.ldx + c0, tail[j]);
+      float nw[V * W];
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        if (j < skip) continue;
-        const int at = len - W + j;              // place of the new window's element j in the sequence; before it, in the old window
-        float nw[V];
-        if (at >= 0) {
-          ldv<V>(p.x, (long long)(begin + at) * p.ldx + c0, p.xt, nw);
-        } else {
+        float x[V];
+        cvt_raw<V, ES>(tail[j], p.xt, x);
 #pragma unroll
-          for (int v = 0; v < V; ++v) nw[v] = old ? st[v * (K - 1) + j + len] : 0.f;      // behind what has been overwritten
+        for (int v = 0; v < V; ++v) {
+          nw[v * W + j] = x[v];
+          if (len - W + j < 0) {
+#pragma unroll
+            for (int i = j + 1; i < W; ++i)
+              if (i == j + len) nw[v * W + j] = was[v * W + i];
+          }
         }
-#pragma unroll
-        for (int v = 0; v < V; ++v) st[v * (K - 1) + j] = nw[v];
       }
+      st_window<W, V>(st, vec_state, nw);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      if (j >= skip) {
-        cvt_raw<V, ES>(wr[j], p.xt, win[j]);
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) win[j][v] = 0.f;
-      }
-    }
+    for (int j = 0; j < W; ++j) cvt_raw<V, ES>(wr[j], p.xt, win[j]);
   }
   // a batch is converted, filtered, activated and stored as a whole: one choice by type for each, none between its loads
   for (int t = t0; t < t1; t += U) {
@@ -178,18 +247,19 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCaus
       for (int v = 0; v < V; ++v) last[j][v] = U - W + j >= 0 ? x[U - W + j >= 0 ? U - W + j : 0][v] : win[j + U < W ? j + U : 0][v];
 #pragma unroll
     for (int u = U - 1; u >= 0; --u)             // newest first: an output takes the place of its input, which only newer outputs saw
+    {
+      float a[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        float a = fmaf(w[W][v], x[u][v], b[v]);
+      for (int v = 0; v < V; ++v) a[v] = b[v];
+      fma_v<V>(a, w[W], x[u]);
 #pragma unroll
-        for (int k = W - 1; k >= 0; --k) a = fmaf(w[k][v], u + k - W >= 0 ? x[u + k - W >= 0 ? u + k - W : 0][v] : win[u + k < W ? u + k : 0][v], a);
-        x[u][v] = a;
-      }
+      for (int k = W - 1; k >= 0; --k) fma_v<V>(a, w[k], u + k - W >= 0 ? x[u + k - W >= 0 ? u + k - W : 0] : win[u + k < W ? u + k : 0]);
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[u][v] = a[v];
+    }
     if (p.act == 1) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int v = 0; v < V; ++v) x[u][v] = silu(x[u][v]);
+      for (int u = 0; u < U; ++u) silu_v<V>(x[u]);
     }
     store_batch<U, V>(p.out, (long long)t * p.ldo + c0, p.ldo, min(U, t1 - t), p.ot, x);
 #pragma unroll
@@ -199,11 +269,9 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCaus
   }
 }
 
-template <int KT, int V, int ES, int RB>
+template <int K, int V, int ES, int RB>
 __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(const MmbCausalConvParams p, int n_groups) {
-  constexpr int W = KT - 1;
-  const int K = KT == 8 ? p.K : KT, skip = KT - K;
-  constexpr bool kVecState = V == 4 && KT < 8;
+  constexpr int W = K - 1;
   pdl_launch_dependents();
   pdl_wait();
   const int g = blockIdx.x * kConvThreads + threadIdx.x;
@@ -213,26 +281,15 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(const Mm
   long long row[RB];
   float win[RB][V * W];
   Raw<V, ES> xr[RB];
-  float w[KT][V], b[V];
-  load_taps<KT, V>(p, c0, K, w, b);
+  float w[K][V], b[V];
+  load_taps<K, V>(p, c0, w, b);
 #pragma unroll
   for (int r = 0; r < RB; ++r) row[r] = r0 + r < p.T ? pool_row(p.rows, r0 + r, p.pool_rows, p.status) : -1;
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
     if (row[r] < 0) continue;
-    const float* st = p.state + (row[r] * p.C + c0) * (K - 1);
-    if constexpr (kVecState) {
-#pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const float4 f = reinterpret_cast<const float4*>(st)[j];
-        win[r][4 * j] = f.x, win[r][4 * j + 1] = f.y, win[r][4 * j + 2] = f.z, win[r][4 * j + 3] = f.w;
-      }
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-#pragma unroll
-        for (int j = 0; j < W; ++j) win[r][v * W + j] = j >= skip ? st[v * (K - 1) + j - skip] : 0.f;
-    }
+    const float* st = p.state + (row[r] * p.C + c0) * W;
+    ld_window<W, V>(st, true, win[r]);
     ld_raw<V, ES>(p.x, (long long)(r0 + r) * p.ldx + c0, xr[r]);
   }
 #pragma unroll
@@ -254,43 +311,54 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(const Mm
         a = fmaf(w[k][v], win[r][v * W + k], a);
         nw[v * W + k] = k + 1 < W ? win[r][v * W + k + 1] : x[v];
       }
-      y[v] = conv_act(a, p.act);
+      y[v] = a;
     }
-    float* st = p.state + (row[r] * p.C + c0) * (K - 1);
-    if constexpr (kVecState) {
+    float s[V];                                      // chosen without a branch, which would end the overlap of the rows (256 rows: 14.6 us against 16.1)
 #pragma unroll
-      for (int j = 0; j < W; ++j) reinterpret_cast<float4*>(st)[j] = make_float4(nw[4 * j], nw[4 * j + 1], nw[4 * j + 2], nw[4 * j + 3]);
-    } else {
+    for (int v = 0; v < V; ++v) s[v] = y[v];
+    silu_v<V>(s);
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-#pragma unroll
-        for (int j = 0; j < W; ++j)
-          if (j >= skip) st[v * (K - 1) + j - skip] = nw[v * W + j];
-    }
+    for (int v = 0; v < V; ++v) y[v] = p.act == 1 ? s[v] : y[v];
+    float* st = p.state + (row[r] * p.C + c0) * W;
+    st_window<W, V>(st, true, nw);
     stv<V>(p.out, (long long)(r0 + r) * p.ldo + c0, p.ot, y);
   }
 }
 
-template <int KT, int V, int ES>
+template <int K, int V, int ES>
 static int launch_conv_v(const MmbCausalConvParams& p, cudaStream_t stream) {
   const int groups = p.C / V;
-  // long tiles read fewer inputs twice and start less often (8111 rows of 10240 channels, us for 8 / 16 / 32 / 64 tokens: 125 / 93 / 78 / 72), short
-  // ones give more threads (500 rows of 2048: 4.5 / 5.8 / 6.6 / 9.5): the longest that leave 2^17 threads
+  static std::atomic<int> resident{0};
+  int ctas = resident.load(std::memory_order_relaxed);
+  if (ctas == 0) {
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, causal_conv_kernel<K, V, ES>, kConvThreads, 0);
+    if (e != cudaSuccess) return (int)e;
+    resident.store(ctas, std::memory_order_relaxed);
+  }
+  // long tiles read fewer inputs twice and start less often (8111 rows of 10240 channels, us for 8 / 16 / 32 / 64 tokens: 128 / 95 / 78 / 72), short
+  // ones give more threads (500 rows of 2048: 4.6 / 5.7 / 7.0 / 10.3): the longest that leave 2^17 threads
   int TT = 8;
   while (TT < 64 && (long long)p.T * groups / (2 * TT) >= (1 << 17)) TT *= 2;
+  // then up to twice that where the last wave is fuller for it; a tile's start costs about six tokens (4096 rows of 8192: 64 tokens, 1.7 waves, 33 us;
+  // 112 tokens, one wave, 30 us)
+  long long best = -1;
+  for (int t = TT, t1 = 2 * TT; t < t1; t += 8) {
+    const long long b = (((long long)p.T + t - 1) / t + p.S / 2) * groups / kConvThreads, cost = (b / (148 * ctas) + (b % (148 * ctas) != 0)) * (t + 6);
+    if (best < 0 || cost < best) best = cost, TT = t;
+  }
   const long long tiles = (long long)p.T / TT + p.S + 2;
   const long long blocks = (tiles * groups + kConvThreads - 1) / kConvThreads;
   if (blocks > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  return launch(causal_conv_kernel<KT, V, ES>, dim3((unsigned)blocks), dim3(kConvThreads), 0, stream, 1, p, groups, TT, tiles);
+  return launch(causal_conv_kernel<K, V, ES>, dim3((unsigned)blocks), dim3(kConvThreads), 0, stream, 1, p, groups, TT, tiles, reinterpret_cast<uintptr_t>(p.state) % 16 == 0);
 }
-template <int KT>
+template <int K>
 static int launch_conv(const MmbCausalConvParams& p, cudaStream_t stream) {
   const bool vec = p.C % 4 == 0 && rows_aligned(p.x, p.ldx, p.xt, 4) && rows_aligned(p.out, p.ldo, p.ot, 4);
-  if (p.xt == 2) return vec ? launch_conv_v<KT, 4, 4>(p, stream) : launch_conv_v<KT, 1, 4>(p, stream);
-  return vec ? launch_conv_v<KT, 4, 2>(p, stream) : launch_conv_v<KT, 1, 2>(p, stream);
+  if (p.xt == 2) return vec ? launch_conv_v<K, 4, 4>(p, stream) : launch_conv_v<K, 1, 4>(p, stream);
+  return vec ? launch_conv_v<K, 4, 2>(p, stream) : launch_conv_v<K, 1, 2>(p, stream);
 }
 
-template <int KT, int V, int ES>
+template <int K, int V, int ES>
 static int launch_conv_step_v(const MmbCausalConvParams& p, cudaStream_t stream) {
   const int groups = p.C / V;
   const unsigned gx = (unsigned)((groups + kConvThreads - 1) / kConvThreads);
@@ -298,15 +366,15 @@ static int launch_conv_step_v(const MmbCausalConvParams& p, cudaStream_t stream)
   const bool many = (long long)groups * p.T >= (1 << 18);
   const long long gy = many ? ((long long)p.T + 3) / 4 : p.T;
   if (gy > 65535) return (int)cudaErrorInvalidValue;
-  if (many) return launch(causal_conv_step_kernel<KT, V, ES, 4>, dim3(gx, (unsigned)gy), dim3(kConvThreads), 0, stream, 1, p, groups);
-  return launch(causal_conv_step_kernel<KT, V, ES, 1>, dim3(gx, (unsigned)gy), dim3(kConvThreads), 0, stream, 1, p, groups);
+  if (many) return launch(causal_conv_step_kernel<K, V, ES, 4>, dim3(gx, (unsigned)gy), dim3(kConvThreads), 0, stream, 1, p, groups);
+  return launch(causal_conv_step_kernel<K, V, ES, 1>, dim3(gx, (unsigned)gy), dim3(kConvThreads), 0, stream, 1, p, groups);
 }
-template <int KT>
+template <int K>
 static int launch_conv_step(const MmbCausalConvParams& p, cudaStream_t stream) {
   const bool vec = p.C % 4 == 0 && rows_aligned(p.x, p.ldx, p.xt, 4) && rows_aligned(p.out, p.ldo, p.ot, 4) &&
                    reinterpret_cast<uintptr_t>(p.state) % 16 == 0;
-  if (p.xt == 2) return vec ? launch_conv_step_v<KT, 4, 4>(p, stream) : launch_conv_step_v<KT, 1, 4>(p, stream);
-  return vec ? launch_conv_step_v<KT, 4, 2>(p, stream) : launch_conv_step_v<KT, 1, 2>(p, stream);
+  if (p.xt == 2) return vec ? launch_conv_step_v<K, 4, 4>(p, stream) : launch_conv_step_v<K, 1, 4>(p, stream);
+  return vec ? launch_conv_step_v<K, 4, 2>(p, stream) : launch_conv_step_v<K, 1, 2>(p, stream);
 }
 
 }  // namespace mmb
@@ -319,6 +387,9 @@ MMB_API int mmb_causal_conv(const MmbCausalConvParams* pp, cudaStream_t stream) 
     case 2: return mmb::launch_conv<2>(p, stream);
     case 3: return mmb::launch_conv<3>(p, stream);
     case 4: return mmb::launch_conv<4>(p, stream);
+    case 5: return mmb::launch_conv<5>(p, stream);
+    case 6: return mmb::launch_conv<6>(p, stream);
+    case 7: return mmb::launch_conv<7>(p, stream);
     default: return mmb::launch_conv<8>(p, stream);
   }
 }
@@ -331,6 +402,9 @@ MMB_API int mmb_causal_conv_step(const MmbCausalConvParams* pp, cudaStream_t str
     case 2: return mmb::launch_conv_step<2>(p, stream);
     case 3: return mmb::launch_conv_step<3>(p, stream);
     case 4: return mmb::launch_conv_step<4>(p, stream);
+    case 5: return mmb::launch_conv_step<5>(p, stream);
+    case 6: return mmb::launch_conv_step<6>(p, stream);
+    case 7: return mmb::launch_conv_step<7>(p, stream);
     default: return mmb::launch_conv_step<8>(p, stream);
   }
 }

@@ -32,11 +32,6 @@ constexpr int kSsmThreads = 128;            // of each role
 constexpr int kSsmTokens = 32;              // of a tile
 constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // log(1 + e^v) = max(v, 0) + log1p(e), e = e^-|v| in (0, 1]: no overflow, and small steps keep their relative accuracy.  log1p(e) / e is smooth on
 // [0, 1] (its singularity lies at -1), so a polynomial of degree 8 fitted to it is within 2^-24.9; with the roundings of its evaluation 2^-22.4.
 __device__ __forceinline__ float softplus(float v) {
@@ -51,29 +46,6 @@ __device__ __forceinline__ float softplus(float v) {
   q = fmaf(q, e, -0.4999949336051941f);
   q = fmaf(q, e, 0.9999999403953552f);
   return fmaf(q, e, fmaxf(v, 0.f));
-}
-
-// Two fp32 values in one 64-bit register: Blackwell multiplies and adds such pairs with one instruction.
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float a, float b) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpack2(f32x2 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
 }
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool ok) {

@@ -283,6 +283,24 @@ def test_conv_in_chunks_and_tokens_equals_one_pass(device, K):
     assert torch.equal(whole, torch.cat(parts)) and torch.equal(one, many) and not one[0].any()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("K", range(2, 9))
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_conv_of_every_number_of_taps(device, K, dtype):
+    """Whole-word rows, sequences shorter and longer than the window, fresh and old; a pool on a 16-byte boundary and one four bytes behind it."""
+    lens, C = [1, 2, 5, 9, 0, 20], 64
+    x, w, b, state, rows, fresh, cu = conv_inputs(device, lens, C, K, TYPES[dtype], seed=K)
+    want = conv_oracle(x, w, b, state, spans(cu, fresh, rows.tolist()), 1)
+    for offset in (0, 1):
+        pool = torch.empty(state.numel() + 1, device=device)[offset:offset + state.numel()].view_as(state).copy_(state)
+        out = ops.causal_conv(x, w, b, cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=device), state=pool, rows=rows.to(device),
+                              fresh=fresh.to(device))
+        check_conv(out, pool, *want)
+        one = torch.empty(state.numel() + 1, device=device)[offset:offset + state.numel()].view_as(state).copy_(state)
+        step = conv_oracle(x[:6], w, b, state, [(i, 1, r, False) for i, r in enumerate(rows.tolist())], 1)
+        check_conv(ops.causal_conv_step(x[:6], w, b, state=one, rows=rows.to(device)), one, *step)
+
+
 SSM_CASES = [
     ([1], 1, 1, "fp32", {}), ([3], 8, 16, "bf16", {}), ([33, 1, 0, 40], 40, 16, "bf16", {"tail": 5}), ([70], 33, 16, "fp16", {}),
     ([5, 66], 24, 8, "fp32", {}), ([31, 7], 16, 24, "bf16", {}), ([65], 48, 64, "bf16", {"bc": torch.float32}), ([20, 9], 17, 128, "fp16", {}),
