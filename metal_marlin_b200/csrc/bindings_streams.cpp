@@ -15,6 +15,9 @@ namespace {
 using torch::Tensor;
 using OptT = c10::optional<Tensor>;
 
+constexpr int64_t kMaxRows = 1 << 30;        // the kernels count rows, sequences and tiles of both in 32 bits
+constexpr int64_t kMaxGrid = 65535;          // rows of a single-token call
+
 inline cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 inline bool given(const OptT& t) { return t.has_value() && t->defined(); }
 inline void check(int err, const char* what) {
@@ -45,13 +48,15 @@ inline const float* opt_f32(const OptT& t, int64_t n, const Tensor& on, const ch
 template <typename P>
 void fill_sequences(P& p, const Tensor& x, const OptT& state, int64_t c, int64_t n, const OptT& rows, const OptT& fresh, const OptT& cu) {
   int64_t S = x.size(0);
-  TORCH_CHECK_VALUE(x.size(0) <= INT_MAX && c <= INT_MAX, "too many rows or channels");
+  TORCH_CHECK_VALUE(x.size(0) <= kMaxRows && c <= INT_MAX, "too many rows or channels");
   if (given(cu)) {
-    TORCH_CHECK_VALUE(cu->scalar_type() == at::kInt && cu->dim() == 1 && cu->numel() >= 1 && cu->numel() <= INT_MAX && cu->is_contiguous() &&
+    TORCH_CHECK_VALUE(cu->scalar_type() == at::kInt && cu->dim() == 1 && cu->numel() >= 1 && cu->numel() <= kMaxRows && cu->is_contiguous() &&
                           cu->device() == x.device(),
                       "cu_seqlens must be a contiguous int32 vector on the device of x");
     S = cu->numel() - 1;
     p.cu_seqlens = cu->data_ptr<int>();
+  } else {
+    TORCH_CHECK_VALUE(S <= kMaxGrid, "a single-token step takes at most ", kMaxGrid, " rows, got ", S);
   }
   if (given(state)) {
     TORCH_CHECK_VALUE(state->scalar_type() == at::kFloat && state->is_contiguous() && state->dim() == 3 && state->size(1) == c && state->size(2) == n,
@@ -179,6 +184,8 @@ void sink_decode(const Tensor& q, const Tensor& k, const Tensor& v, const OptT& 
   TORCH_CHECK_VALUE(block_tables.dim() == 2 && block_tables.size(0) == B && block_tables.scalar_type() == at::kInt && block_tables.is_contiguous() &&
                         ctx_lens.scalar_type() == at::kInt && ctx_lens.is_contiguous(),
                     "block_tables [B, blocks] and ctx_lens [B] must be contiguous int32");
+  TORCH_CHECK_VALUE(B <= kMaxGrid, "attention with sinks takes at most ", kMaxGrid, " rows, got ", B);
+  TORCH_CHECK_VALUE(block_tables.size(1) <= kMaxRows / block_size, "block_tables reaches more than ", kMaxRows, " tokens");
   TORCH_CHECK_VALUE(fmt >= -1 && fmt <= 3, "unknown cache format");
   const int64_t row = fmt >= 2 ? D / 2 : D;
   TORCH_CHECK_VALUE(k.scalar_type() == (fmt < 0 ? at::kBFloat16 : at::kByte) && v.scalar_type() == k.scalar_type(), "K and V pools have another type");

@@ -569,6 +569,9 @@ def _sink_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv,
             raise ValueError(f"attention with sinks takes head sizes 64, 128 and 256, got {dv}")
         if Hkv < 1 or Hq % Hkv:
             raise ValueError("query heads must be a multiple of KV heads")
+        if B > 65535 or block_size < 1 or block_tables.shape[1] > (1 << 30) // block_size:
+            raise ValueError(f"attention with sinks takes at most 65535 rows and tables of at most 2^30 tokens, got {B} rows of "
+                             f"{block_tables.shape[1]} blocks of {block_size}")
         if quant:
             k_pool, v_pool = k_pool.dequantize(), v_pool.dequantize()
         o = ref.paged_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv, block_size, scale, window, sinks)
@@ -604,6 +607,8 @@ def _stream_out(x, out, out_dtype, *inputs):
         return torch.empty_like(x) if out_dtype is None else torch.empty_like(x, dtype=out_dtype)
     if out_dtype is not None and out.dtype != out_dtype:
         raise ValueError(f"out is {out.dtype}, out_dtype {out_dtype}")
+    if out.dim() == 2 and out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+        raise ValueError("the rows of out must not overlap")
     for t in inputs:
         if t is None or t.numel() == 0 or out.numel() == 0 or t.untyped_storage().data_ptr() != out.untyped_storage().data_ptr():
             continue

@@ -219,6 +219,8 @@ def _sequences(x, state, c, n, rows, fresh, cu):
         _need(cu.dtype == torch.int32 and cu.dim() == 1 and cu.numel() >= 1 and cu.is_contiguous() and cu.device == x.device,
               "cu_seqlens must be a contiguous int32 vector on the device of x")
         S = cu.numel() - 1
+    else:
+        _need(S <= 65535, f"a single-token step takes at most 65535 rows, got {S}")
     if state is not None:
         _need(state.dtype == torch.float32 and state.is_contiguous() and state.dim() == 3 and tuple(state.shape[1:]) == (c, n),
               f"state must be a contiguous fp32 pool [rows, {c}, {n}]")

@@ -761,3 +761,42 @@ def test_a_stream_through_all_of_them(device):
     order = torch.cat([torch.arange(int(i) * bs, int(i) * bs + bs) for i in table[0]])
     for t, o in zip(range(40, T), os_):
         check_attention(o, attention_oracle(q[t: t + 1], kp.double().cpu()[order], vp.double().cpu()[order], torch.arange(4)[None], [t + 1], Hkv, bs, D ** -0.5, window, sinks))
+
+
+def test_refusals_of_calls_that_are_too_large_or_write_a_row_twice():
+    """Expanded tensors: nothing of that size is allocated."""
+    from metal_marlin_b200 import _build
+    native = _build.load()
+    x, w = torch.zeros(1, 4).expand(65536, 4), torch.zeros(4, 2)
+    state = torch.zeros(1, 4, 1)
+    rows = torch.full((65536,), -1)
+    with pytest.raises(ValueError):
+        ops.causal_conv_step(x, w, state=state, rows=rows)
+    A, bc = torch.zeros(4, 3), torch.zeros(1, 3).expand(65536, 3)
+    with pytest.raises(ValueError):
+        ops.ssm_step(x, x, A, bc, bc, state=torch.zeros(1, 4, 3), rows=rows)
+    cu = torch.tensor([0, 5], dtype=torch.int32)
+    with pytest.raises(ValueError):
+        ops.causal_conv(x[:5].clone(), w, cu_seqlens=cu, out=torch.zeros(1, 4).expand(5, 4))
+    wide = torch.zeros(8)
+    with pytest.raises(ValueError):
+        ops.causal_conv(x[:5].clone(), w, cu_seqlens=cu, out=wide.as_strided((5, 4), (1, 1)))
+    pool, q = torch.zeros(16, 1, 64, dtype=torch.bfloat16), torch.zeros(1, 1, 64, dtype=torch.bfloat16)
+    base = dict(Hq=1, Hkv=1, dqk=64, dv=64, scale=1.0, window=8, sinks=2)
+    lens = torch.zeros(1, dtype=torch.int32)
+    for bs, n in ((2 ** 30, 2), (2 ** 31 - 1, 1), (16, 2 ** 26 + 1)):
+        tables = torch.zeros(1, n, dtype=torch.int32) if n < 100 else torch.zeros(1, 1, dtype=torch.int32).expand(1, n)
+        with pytest.raises(ValueError):
+            ops.paged_attention(q, pool, pool, tables, lens, block_size=bs, **base)
+        if native and n < 100:
+            with pytest.raises(ValueError):
+                torch.ops.mmb200.sink_decode(q, pool, pool, None, None, tables, lens, q.clone(), 1, 1, 64, bs, 1.0, 8, 2, -1, 0)
+    many = torch.zeros(65536, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        ops.paged_attention(q.expand(65536, 1, 64), pool, pool, torch.zeros(65536, 1, dtype=torch.int32), many, block_size=16, **base)
+    if native:
+        with pytest.raises(ValueError):
+            torch.ops.mmb200.causal_conv(x, w, None, torch.empty(65536, 4), state, rows, None, None, 1, True)
+        with pytest.raises(ValueError):
+            torch.ops.mmb200.sink_decode(q.expand(65536, 1, 64).contiguous(), pool, pool, None, None, torch.zeros(65536, 1, dtype=torch.int32), many,
+                                         torch.empty(65536, 1, 64, dtype=torch.bfloat16), 1, 1, 64, 16, 1.0, 8, 2, -1, 0)
