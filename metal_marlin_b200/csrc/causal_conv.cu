@@ -140,9 +140,8 @@ __device__ __forceinline__ void store_batch(void* out, long long at, long long l
   }
 }
 
-template <int K, int V, int ES>
+template <int K, int V, int ES, int U>
 __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCausalConvParams p, int n_groups, int TT, long long n_tiles, bool vec_state) {
-  constexpr int U = V == 4 && ES == 4 ? 4 : 8;             // tokens loaded together
   constexpr int W = K - 1;
   pdl_launch_dependents();
   pdl_wait();
@@ -325,13 +324,13 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_step_kernel(const Mm
   }
 }
 
-template <int K, int V, int ES>
-static int launch_conv_v(const MmbCausalConvParams& p, cudaStream_t stream) {
+template <int K, int V, int ES, int U>
+static int launch_conv_u(const MmbCausalConvParams& p, cudaStream_t stream) {
   const int groups = p.C / V;
   static std::atomic<int> resident{0};
   int ctas = resident.load(std::memory_order_relaxed);
   if (ctas == 0) {
-    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, causal_conv_kernel<K, V, ES>, kConvThreads, 0);
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, causal_conv_kernel<K, V, ES, U>, kConvThreads, 0);
     if (e != cudaSuccess) return (int)e;
     resident.store(ctas, std::memory_order_relaxed);
   }
@@ -349,7 +348,19 @@ static int launch_conv_v(const MmbCausalConvParams& p, cudaStream_t stream) {
   const long long tiles = (long long)p.T / TT + p.S + 2;
   const long long blocks = (tiles * groups + kConvThreads - 1) / kConvThreads;
   if (blocks > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-  return launch(causal_conv_kernel<K, V, ES>, dim3((unsigned)blocks), dim3(kConvThreads), 0, stream, 1, p, groups, TT, tiles, reinterpret_cast<uintptr_t>(p.state) % 16 == 0);
+  return launch(causal_conv_kernel<K, V, ES, U>, dim3((unsigned)blocks), dim3(kConvThreads), 0, stream, 1, p, groups, TT, tiles, reinterpret_cast<uintptr_t>(p.state) % 16 == 0);
+}
+// U: tokens a thread loads together
+template <int K, int V, int ES>
+static int launch_conv_v(const MmbCausalConvParams& p, cudaStream_t stream) {
+  constexpr int U = V == 4 && ES == 4 ? 4 : 8;
+  if constexpr (V == 4 && ES == 2) {
+    // short sequences are mostly starts: smaller batches take fewer registers, so more starts overlap (8192 channels, us for U = 8 / 4 / 2: 155 sequences
+    // of 1 to 20 tokens 28 / 21 / 20, 64 of 20 to 40 tokens 30 / 27 / 28; 300 single tokens of 10240: 57 / 40 / 32; one prompt of 4096: 29 / 33 / -)
+    if (p.S > 1 && p.T / p.S <= 8) return launch_conv_u<K, V, ES, 2>(p, stream);
+    if (p.S > 1 && p.T / p.S <= 32) return launch_conv_u<K, V, ES, 4>(p, stream);
+  }
+  return launch_conv_u<K, V, ES, U>(p, stream);
 }
 template <int K>
 static int launch_conv(const MmbCausalConvParams& p, cudaStream_t stream) {

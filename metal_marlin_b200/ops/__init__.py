@@ -597,6 +597,8 @@ _reporting = set()
 def _report_on(device) -> None:
     """Registers the device's status word on first use (kernels report bad block tables and pool rows there)."""
     if device not in _reporting:
+        if str(device) not in _status and torch.cuda.is_current_stream_capturing():
+            return                              # the word would live in the graph's memory; the next call outside a capture registers it
         gemm_status(device)
         _reporting.add(device)
 
