@@ -41,11 +41,6 @@ __device__ __forceinline__ void fma_v(float (&a)[V], const float (&w)[V], const 
     for (int v = 0; v < V; ++v) a[v] = fmaf(w[v], x[v], a[v]);
   }
 }
-__device__ __forceinline__ float rcp_fast(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // x / (1 + e^-x)
 template <int V>
 __device__ __forceinline__ void silu_v(float (&x)[V]) {

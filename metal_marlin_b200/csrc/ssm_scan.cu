@@ -9,14 +9,14 @@
 // 32 bytes a clock that shared memory returns to each scheduler's registers (8 bytes of B and C a state).  The recurrence itself is one
 // multiply-add deep.  The work is split over channels and over the STATES of a channel, never over time (a second pass over time would
 // double the exponentials): S lanes share a channel, each with NPL states in registers (of R channels where there are lanes to spare).  A block
-// owns 128 / S R channels of one sequence and walks it in tiles of 32 tokens with two roles that meet at named barriers, tile by tile:
-//   * four staging warps: the tile's x, dt, z, B, C arrive raw by 16-byte cp.async two tiles ahead; they turn x and dt into (d, d x) pairs, so softplus
-//     is paid once per value and not once per lane, and later add the skip term, apply the gate and store the outputs;
-//   * four scanning warps: G tokens at a time, all their exponentials before the recurrence, the next group's loads before both; partial sums of S
+// owns 32 W / S R channels of one sequence and walks it in tiles of 32 or 64 tokens with two roles that meet at named barriers, tile by tile:
+//   * ST / 32 staging warps: the tile's x, dt, z, B, C arrive raw by 16-byte cp.async two tiles ahead; they turn x and dt into (d, d x) pairs, so
+//     softplus is paid once per value and not once per lane, and later add the skip term, apply the gate and store the outputs;
+//   * W scanning warps: G tokens at a time, all their exponentials before the recurrence, the next group's loads before both; partial sums of S
 //     tokens are added over the S lanes by a transposing butterfly (S - 1 shuffles for S tokens) that leaves every lane with the sum of one token.
 // What it took (4096 tokens of 8192 channels, 16 states, bf16): one role with runtime types 1132 us; blocks spread evenly over the SMs and loads of a
 // batch issued before their conversions 772 -> 547; types at compile time, conflict-free staging 386; the two roles 327; groups of four
-// tokens, unrolled 262 us.
+// tokens, unrolled 262; seven scanning warps on every SM instead of eight on most 244 us.
 // exp(d A) is taken as 2^(d (A log2 e)); A log2 e is rounded once, which shifts every exponent by the same relative 2^-24.
 //
 // Single tokens.  The state is the traffic: see ssm_step_kernel.
@@ -28,8 +28,7 @@
 
 namespace mmb {
 
-constexpr int kSsmThreads = 128;            // of each role
-constexpr int kSsmTokens = 32;              // of a tile
+constexpr int kStepThreads = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // log(1 + e^v) = max(v, 0) + log1p(e), e = e^-|v| in (0, 1]: no overflow, and small steps keep their relative accuracy.  log1p(e) / e is smooth on
@@ -54,6 +53,32 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool ok) 
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// softplus of two values; the polynomial takes one instruction a step for both.
+__device__ __forceinline__ void softplus2(float (&v)[2]) {
+  const float e0 = exp2_fast(-kLog2e * fabsf(v[0])), e1 = exp2_fast(-kLog2e * fabsf(v[1]));
+  const f32x2 e = pack2(e0, e1);
+  auto both = [](float c) { return pack2(c, c); };
+  f32x2 q = both(0.0052326880395412445f);
+  q = fma2(q, e, both(-0.029505213722586632f));
+  q = fma2(q, e, both(0.07822591066360474f));
+  q = fma2(q, e, both(-0.13663242757320404f));
+  q = fma2(q, e, both(0.19106005132198334f));
+  q = fma2(q, e, both(-0.2484298199415207f));
+  q = fma2(q, e, both(0.3331909775733948f));
+  q = fma2(q, e, both(-0.4999949336051941f));
+  q = fma2(q, e, both(0.9999999403953552f));
+  const float2 f = unpack2(fma2(q, e, pack2(fmaxf(v[0], 0.f), fmaxf(v[1], 0.f))));
+  v[0] = f.x, v[1] = f.y;
+}
+// y silu(z) for two values
+__device__ __forceinline__ void gate2(float (&y)[2], const float (&z)[2]) {
+  const f32x2 zz = pack2(z[0], z[1]);
+  float2 f = unpack2(mul2(zz, pack2(-kLog2e, -kLog2e)));
+  f = unpack2(add2(pack2(exp2_fast(f.x), exp2_fast(f.y)), pack2(1.f, 1.f)));
+  f = unpack2(mul2(mul2(zz, pack2(rcp_fast(f.x), rcp_fast(f.y))), pack2(y[0], y[1])));
+  y[0] = f.x, y[1] = f.y;
+}
 
 // Sums v[i] over the S lanes of a group for i < S; lane s of the group ends with the sums of v[s] in v[0].
 template <int S, int R>
@@ -140,6 +165,8 @@ struct SsmLayout {
   int x, dt, z, b, c, stage, step, bf, cf, y, total;
 };
 constexpr int kSsmStages = 3;               // raw tiles: one arriving, one being prepared, one whose outputs are being finished
+// Row pitch of the partial outputs: eight more than a multiple of 32 spreads the tokens that a warp writes at once over the banks.
+__host__ __device__ constexpr int ssm_y_pitch(int CH) { return CH < 32 ? CH + 8 : (CH + 31) / 32 * 32 + 8; }
 __host__ __device__ inline SsmLayout ssm_layout(int TT, int CH, int NP, int xb, int dtb, int zb, int bb) {
   SsmLayout l;
   int at = 0;
@@ -154,7 +181,7 @@ __host__ __device__ inline SsmLayout ssm_layout(int TT, int CH, int NP, int xb, 
   l.step = at, at += 2 * TT * CH * 8;       // {d, d x}
   l.bf = at, at += bb == 4 ? 0 : 2 * TT * NP * 4;   // fp32 tiles are used where they arrive
   l.cf = at, at += bb == 4 ? 0 : 2 * TT * NP * 4;
-  l.y = at, at += 2 * TT * (CH + 8) * 4;    // the padding spreads the tokens that a warp writes at once over the banks
+  l.y = at, at += 2 * TT * ssm_y_pitch(CH) * 4;
   l.total = at;
   return l;
 }
@@ -171,10 +198,11 @@ template <int ID, int N>
 __device__ __forceinline__ void bar_arrive_of(int buffer) { buffer ? bar_arrive<ID + 1, N>() : bar_arrive<ID, N>(); }
 
 // XT: the type of x, dt, z, B, C and out where they have one type, else 3.
-template <int S, int NPL, int R, int G, int XT>
-__global__ void __launch_bounds__(2 * kSsmThreads) ssm_scan_kernel(const MmbSsmParams p, int n_blocks, int vec_x, int vec_bc, int vec_out) {
+// W: scanning warps; ST: staging threads; TT: tokens of a tile.
+template <int S, int NPL, int R, int G, int W, int ST, int TT, int XT>
+__global__ void __launch_bounds__(32 * W + ST) ssm_scan_kernel(const MmbSsmParams p, int n_blocks, int vec_x, int vec_bc, int vec_out) {
   const int xt = XT < 3 ? XT : p.xt, dtt = XT < 3 ? XT : p.dtt, zt = XT < 3 ? XT : p.zt, bt = XT < 3 ? XT : p.bt, ot = XT < 3 ? XT : p.ot;
-  constexpr int CH = kSsmThreads / S * R, TT = kSsmTokens, NP = S * NPL, YS = CH + 8;
+  constexpr int CH = 32 * W / S * R, NP = S * NPL, YS = ssm_y_pitch(CH), kScan = 32 * W, kAll = kScan + ST;
   constexpr int SG = 2 * G > S ? 2 * G : S;                 // tokens between two sums over the lanes: an even number of groups
   extern __shared__ __align__(16) unsigned char sm[];
   const int seq = blockIdx.x / n_blocks, c0 = (blockIdx.x % n_blocks) * CH;
@@ -189,7 +217,7 @@ __global__ void __launch_bounds__(2 * kSsmThreads) ssm_scan_kernel(const MmbSsmP
   }
   if (!live) {                                    // rows of no live sequence
     if (p.zero_dead)
-      for (long long i = threadIdx.x; i < (long long)(end - begin) * CH; i += 2 * kSsmThreads) {
+      for (long long i = threadIdx.x; i < (long long)(end - begin) * CH; i += kAll) {
         const int c = c0 + (int)(i % CH);
         if (c < p.D) st1(p.out, (begin + i / CH) * p.ldo + c, ot, 0.f);
       }
@@ -199,22 +227,22 @@ __global__ void __launch_bounds__(2 * kSsmThreads) ssm_scan_kernel(const MmbSsmP
   const SsmLayout L = ssm_layout(TT, CH, NP, xb, dtb, zb, bb);
   const int tiles = (end - begin + TT - 1) / TT;
 
-  if (threadIdx.x >= kSsmThreads) {
+  if (threadIdx.x >= kScan) {
     // ------------------------------------------------------------------------------------------------ staging warps
-    const int tid = threadIdx.x - kSsmThreads;
-    // rows t0 .. t0 + TT of COLS columns (a power of two) of a [*, width] tensor into a dense raw tile; zeros outside.  16-byte pieces where the
+    const int tid = threadIdx.x - kScan;
+    // rows t0 .. t0 + TT of COLS columns of a [*, width] tensor into a dense raw tile; zeros outside.  16-byte pieces where the
     // rows are aligned for it: a thread's pieces lie in one column of pieces, so its addresses are one pointer and a stride.
     auto fetch16 = [&](auto cols, auto es, unsigned char* dst, const unsigned char* src, long long ld, int width, int t0) {
-      constexpr int COLS = decltype(cols)::value, ES = decltype(es)::value, PER = COLS * ES / 16, PIECES = TT * PER;
+      constexpr int COLS = decltype(cols)::value, ES = decltype(es)::value, PER = COLS * ES / 16, RS = ST / PER;   // pieces a row, rows a pass
       const int r0 = tid / PER, q = tid % PER;
       const bool in = q * (16 / ES) < width;
       const unsigned char* g = src + (t0 + r0) * ld * ES + q * 16;
 #pragma unroll
-      for (int k = 0; k < (PIECES + kSsmThreads - 1) / kSsmThreads; ++k) {
-        const int r = r0 + k * (kSsmThreads / PER);
-        if (PIECES % kSsmThreads == 0 || r < TT) {
+      for (int k = 0; k < (TT + RS - 1) / RS; ++k) {
+        const int r = r0 + k * RS;
+        if ((ST % PER == 0 || r0 < RS) && (TT % RS == 0 || r < TT)) {
           const bool ok = in && t0 + r < end;
-          cp_async16(dst + (tid + k * kSsmThreads) * 16, ok ? g + k * (kSsmThreads / PER) * ld * ES : src, ok);
+          cp_async16(dst + (r * PER + q) * 16, ok ? g + k * RS * ld * ES : src, ok);
         }
       }
     };
@@ -222,12 +250,16 @@ __global__ void __launch_bounds__(2 * kSsmThreads) ssm_scan_kernel(const MmbSsmP
       constexpr int COLS = decltype(cols)::value;
       const unsigned char* src = reinterpret_cast<const unsigned char*>(base) + (long long)col * es;
       width -= col;
-      if (vec) {
-        if (es == 2) fetch16(cols, Int<2>{}, dst, src, ld, width, t0);
-        else fetch16(cols, Int<4>{}, dst, src, ld, width, t0);
+      if (vec && COLS * es % 16 == 0) {
+        if constexpr (COLS * 2 % 16 == 0) {
+          if (es == 2) fetch16(cols, Int<2>{}, dst, src, ld, width, t0);
+        }
+        if constexpr (COLS * 4 % 16 == 0) {
+          if (es == 4) fetch16(cols, Int<4>{}, dst, src, ld, width, t0);
+        }
         return;
       }
-      for (int i = tid; i < TT * COLS; i += kSsmThreads) {
+      for (int i = tid; i < TT * COLS; i += ST) {
         const int r = i / COLS, q = i % COLS;
         const bool ok = t0 + r < end && q < width;
         const long long at = (long long)(t0 + r) * ld + q;
@@ -250,8 +282,11 @@ __global__ void __launch_bounds__(2 * kSsmThreads) ssm_scan_kernel(const MmbSsmP
     prefetch(0);
     prefetch(1);
     // this thread's values of a tile: channels vc, vc + 1 of the tokens vt, vt + VS, ..
-    constexpr int VS = 2 * kSsmThreads / CH, VN = TT / VS;
+    constexpr int VS = ST / (CH / 2), VN = (TT + VS - 1) / VS;
+    constexpr bool kEven = ST % (CH / 2) == 0 && TT % VS == 0;            // every thread has VN tokens
     const int vt = tid / (CH / 2), vc = tid % (CH / 2) * 2;
+    auto mine = [&](int k) { return kEven || (vt < VS && vt + k * VS < TT); };
+    auto at = [&](int k) { return kEven ? vt + k * VS : min(vt + k * VS, TT - 1); };
     float bias[2], skip[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -265,22 +300,23 @@ __global__ void __launch_bounds__(2 * kSsmThreads) ssm_scan_kernel(const MmbSsmP
       float x[VN][2], d[VN][2];
 #pragma unroll
       for (int k = 0; k < VN; ++k) {
-        ld2(st + L.x, (vt + k * VS) * CH + vc, xt, x[k]);
-        ld2(st + L.dt, (vt + k * VS) * CH + vc, dtt, d[k]);
+        ld2(st + L.x, at(k) * CH + vc, xt, x[k]);
+        ld2(st + L.dt, at(k) * CH + vc, dtt, d[k]);
       }
 #pragma unroll
       for (int k = 0; k < VN; ++k) d[k][0] += bias[0], d[k][1] += bias[1];
       if (p.softplus) {
 #pragma unroll
-        for (int k = 0; k < VN; ++k) d[k][0] = softplus(d[k][0]), d[k][1] = softplus(d[k][1]);
+        for (int k = 0; k < VN; ++k) softplus2(d[k]);
       }
       float4* step = reinterpret_cast<float4*>(sm + L.step + (i & 1) * TT * CH * 8);
 #pragma unroll
-      for (int k = 0; k < VN; ++k) step[((vt + k * VS) * CH + vc) / 2] = make_float4(d[k][0], d[k][0] * x[k][0], d[k][1], d[k][1] * x[k][1]);
+      for (int k = 0; k < VN; ++k)
+        if (mine(k)) step[((vt + k * VS) * CH + vc) / 2] = make_float4(d[k][0], d[k][0] * x[k][0], d[k][1], d[k][1] * x[k][1]);
       if (bb == 2) {
         float4* bf = reinterpret_cast<float4*>(sm + L.bf) + (i & 1) * TT * NP / 4;
         float4* cf = reinterpret_cast<float4*>(sm + L.cf) + (i & 1) * TT * NP / 4;
-        for (int q = tid; q < TT * NP / 4; q += kSsmThreads) {
+        for (int q = tid; q < TT * NP / 4; q += ST) {
           float v[4];
           ldv<4>(st + L.b, 4 * q, bt, v);
           bf[q] = make_float4(v[0], v[1], v[2], v[3]);
@@ -297,8 +333,8 @@ __global__ void __launch_bounds__(2 * kSsmThreads) ssm_scan_kernel(const MmbSsmP
       float x[VN][2], y[VN][2];
 #pragma unroll
       for (int k = 0; k < VN; ++k) {
-        ld2(st + L.x, (vt + k * VS) * CH + vc, xt, x[k]);
-        const float2 f = *reinterpret_cast<const float2*>(yt + (vt + k * VS) * YS + vc);
+        ld2(st + L.x, at(k) * CH + vc, xt, x[k]);
+        const float2 f = *reinterpret_cast<const float2*>(yt + at(k) * YS + vc);
         y[k][0] = f.x, y[k][1] = f.y;
       }
 #pragma unroll
@@ -306,13 +342,13 @@ __global__ void __launch_bounds__(2 * kSsmThreads) ssm_scan_kernel(const MmbSsmP
       if (p.z) {
         float z[VN][2];
 #pragma unroll
-        for (int k = 0; k < VN; ++k) ld2(st + L.z, (vt + k * VS) * CH + vc, zt, z[k]);
+        for (int k = 0; k < VN; ++k) ld2(st + L.z, at(k) * CH + vc, zt, z[k]);
 #pragma unroll
-        for (int k = 0; k < VN; ++k) y[k][0] *= silu(z[k][0]), y[k][1] *= silu(z[k][1]);
+        for (int k = 0; k < VN; ++k) gate2(y[k], z[k]);
       }
 #pragma unroll
       for (int k = 0; k < VN; ++k) {
-        if (t0 + vt + k * VS < end) {
+        if (mine(k) && t0 + vt + k * VS < end) {
           const long long at = (long long)(t0 + vt + k * VS) * p.ldo + c0 + vc;
           if (vec_out) {
             if (c0 + vc < p.D) st2(p.out, at, ot, y[k]);
@@ -325,17 +361,17 @@ __global__ void __launch_bounds__(2 * kSsmThreads) ssm_scan_kernel(const MmbSsmP
     };
     for (int i = 0; i < tiles; ++i) {
       cp_async_wait<1>();
-      bar_sync<kBarStage, kSsmThreads>();           // raw tile i is there
+      bar_sync<kBarStage, ST>();           // raw tile i is there
       prepare(i);
-      bar_arrive_of<kBarFull, 2 * kSsmThreads>(i & 1);
+      bar_arrive_of<kBarFull, kAll>(i & 1);
       if (i > 0) {
-        bar_sync_of<kBarDone, 2 * kSsmThreads>((i - 1) & 1);
+        bar_sync_of<kBarDone, kAll>((i - 1) & 1);
         finish(i - 1);
       }
-      bar_sync<kBarStage, kSsmThreads>();           // everybody is done with raw tile i - 1
+      bar_sync<kBarStage, ST>();           // everybody is done with raw tile i - 1
       prefetch(i + 2);
     }
-    bar_sync_of<kBarDone, 2 * kSsmThreads>((tiles - 1) & 1);
+    bar_sync_of<kBarDone, kAll>((tiles - 1) & 1);
     finish(tiles - 1);
     return;
   }
@@ -410,7 +446,7 @@ __global__ void __launch_bounds__(2 * kSsmThreads) ssm_scan_kernel(const MmbSsmP
     const float* bp = (bb == 4 ? reinterpret_cast<const float*>(sm + i % kSsmStages * L.stage + L.b) : reinterpret_cast<const float*>(sm + L.bf) + (i & 1) * TT * NP) + s * NPL;
     const float* cp = (bb == 4 ? reinterpret_cast<const float*>(sm + i % kSsmStages * L.stage + L.c) : reinterpret_cast<const float*>(sm + L.cf) + (i & 1) * TT * NP) + s * NPL;
     float* yt = reinterpret_cast<float*>(sm + L.y) + (i & 1) * TT * YS + s * YS + cl;
-    bar_sync_of<kBarFull, 2 * kSsmThreads>(i & 1);
+    bar_sync_of<kBarFull, kAll>(i & 1);
     if (valid == TT) {
       Loaded ld[2];
       load(step, bp, cp, 0, ld[0]);
@@ -436,7 +472,7 @@ __global__ void __launch_bounds__(2 * kSsmThreads) ssm_scan_kernel(const MmbSsmP
         emit<S, R, SG, YS>(v, s, yt + t * YS);
       }
     }
-    bar_arrive_of<kBarDone, 2 * kSsmThreads>(i & 1);
+    bar_arrive_of<kBarDone, kAll>(i & 1);
   }
   if (p.state) {
 #pragma unroll
@@ -490,9 +526,9 @@ __device__ __forceinline__ uint32_t ld_bits(const void* p, long long i, int t) {
 // repeats: two pieces a lane instead of one are worth 78 -> 51 us together with the walk along the row (256 rows of 8192 channels, 16 states: 5.6 TB/s;
 // walking the rows of one group of channels with A in registers instead, 65 us: the accesses of neighbouring blocks lie further apart).
 template <int S, int PCS, int XT>
-__global__ void __launch_bounds__(kSsmThreads) ssm_step_kernel(const MmbSsmParams p, int per) {
+__global__ void __launch_bounds__(kStepThreads) ssm_step_kernel(const MmbSsmParams p, int per) {
   const int xt = XT < 3 ? XT : p.xt, dtt = XT < 3 ? XT : p.dtt, zt = XT < 3 ? XT : p.zt, bt = XT < 3 ? XT : p.bt;
-  constexpr int CB = kSsmThreads / S;
+  constexpr int CB = kStepThreads / S;
   const int lane = threadIdx.x % S, N = p.N, t = blockIdx.y;
   const int ch0 = blockIdx.x * per * CB + threadIdx.x / S;
   pdl_launch_dependents();
@@ -593,9 +629,9 @@ static int allow_smem(F kernel, int bytes, std::atomic<unsigned long long>& done
   return (int)e;
 }
 
-template <int S, int NPL, int R, int G, int XT>
+template <int S, int NPL, int R, int G, int W, int ST, int TT, int XT>
 static int launch_scan_t(const MmbSsmParams& p, cudaStream_t stream) {
-  constexpr int CH = kSsmThreads / S * R, TT = kSsmTokens;
+  constexpr int CH = 32 * W / S * R;
   const bool vx = p.D % 8 == 0 && rows_aligned(p.x, p.ldx, p.xt, 8) && rows_aligned(p.dt, p.lddt, p.dtt, 8) && rows_aligned(p.z, p.ldz, p.zt, 8);
   const bool vb = (p.N * elt_bytes(p.bt)) % 16 == 0 && rows_aligned(p.B, p.ldb, p.bt, 8) && rows_aligned(p.C, p.ldc, p.bt, 8);
   const bool vo = p.D % 2 == 0 && rows_aligned(p.out, p.ldo, p.ot, 2);
@@ -608,28 +644,54 @@ static int launch_scan_t(const MmbSsmParams& p, cudaStream_t stream) {
   const long long share = ((long long)nb * p.S + 147) / 148;
   if (share >= 1 && share <= 4) smem = max(smem, (size_t)(kSmem / share - 1024) / 128 * 128);
   static std::atomic<unsigned long long> done{0};
-  const int e = allow_smem(ssm_scan_kernel<S, NPL, R, G, XT>, kSmem, done);
+  const int e = allow_smem(ssm_scan_kernel<S, NPL, R, G, W, ST, TT, XT>, kSmem, done);
   if (e) return e;
   // not a programmatic dependent launch: blocks that start while the previous kernel drains pile up on the SMs that it leaves first, and a scan
   // has too few blocks to even that out
-  ssm_scan_kernel<S, NPL, R, G, XT><<<(unsigned)blocks, 2 * kSsmThreads, smem, stream>>>(p, nb, (int)vx, (int)vb, (int)vo);
+  ssm_scan_kernel<S, NPL, R, G, W, ST, TT, XT><<<(unsigned)blocks, 32 * W + ST, smem, stream>>>(p, nb, (int)vx, (int)vb, (int)vo);
   return (int)cudaGetLastError();
 }
+template <int S, int NPL, int R, int G, int W, int ST, int TT>
+static int launch_scan_w(const MmbSsmParams& p, cudaStream_t stream) {
+  return p.xt == 0   ? launch_scan_t<S, NPL, R, G, W, ST, TT, 0>(p, stream)
+         : p.xt == 1 ? launch_scan_t<S, NPL, R, G, W, ST, TT, 1>(p, stream)
+                     : launch_scan_t<S, NPL, R, G, W, ST, TT, 2>(p, stream);
+}
+// Blocks of four scanning warps, unless some SMs would get two of them where wider blocks give every SM at most one: then the SM with the most
+// work has W warps instead of eight.  A block that has its SM to itself needs more staging warps, or they are what the scan waits for, and the wide
+// ones longer tiles, as there is no other block to run while the two roles hand over.  Measured (bf16, 16 states; us for four and for W warps):
+// 4096 tokens of 8192 channels 263 / 244 (7), 2048 of 7000 136 / 117 (6), 2048 of 5120 134 / 112 (5); 64 states, 1531 of 1536, fp32 95 / 82 (6).  One
+// block of four warps an SM, with four and with eight staging warps: 2048 of 4096 94 / 84, 4096 of 1536 (eight lanes a channel) 134 / 129.
 template <int S, int NPL, int R, int G>
 static int launch_scan(const MmbSsmParams& p, cudaStream_t stream) {
   const bool same = p.dtt == p.xt && p.bt == p.xt && p.ot == p.xt && (p.z == nullptr || p.zt == p.xt);
-  if (!same) return launch_scan_t<S, NPL, R, G, 3>(p, stream);
-  return p.xt == 0 ? launch_scan_t<S, NPL, R, G, 0>(p, stream) : p.xt == 1 ? launch_scan_t<S, NPL, R, G, 1>(p, stream) : launch_scan_t<S, NPL, R, G, 2>(p, stream);
+  if (!same) return launch_scan_t<S, NPL, R, G, 4, 128, 32, 3>(p, stream);
+  constexpr int PER = 32 / S * R;                  // channels a warp
+  auto one_each = [&](int warps) { return ((long long)p.D + warps * PER - 1) / (warps * PER) * p.S <= 148; };
+  if constexpr (S == 4 && NPL == 4) {
+    if (one_each(4)) return launch_scan_w<S, NPL, R, G, 4, 256, 32>(p, stream);
+    if (one_each(5)) return launch_scan_w<S, NPL, R, G, 5, 384, 64>(p, stream);
+    if (one_each(6)) return launch_scan_w<S, NPL, R, G, 6, 384, 64>(p, stream);
+    // in fp32 a tile of seven warps does not fit the shared memory
+    if (p.xt != 2 && one_each(7)) return launch_scan_w<S, NPL, R, G, 7, 256, 64>(p, stream);
+  }
+  if constexpr (S == 8 && NPL == 2) {
+    if (one_each(4)) return launch_scan_w<S, NPL, R, G, 4, 256, 32>(p, stream);
+  }
+  if constexpr (S == 16 && NPL == 4 && R == 1) {
+    if (!one_each(4) && one_each(6)) return launch_scan_w<S, NPL, R, G, 6, 384, 64>(p, stream);
+  }
+  return launch_scan_w<S, NPL, R, G, 4, 128, 32>(p, stream);
 }
 
 template <int S, int PCS, int XT>
 static int launch_step_t(const MmbSsmParams& p, cudaStream_t stream) {
-  const int groups = (p.D + kSsmThreads / S - 1) / (kSsmThreads / S);
+  const int groups = (p.D + kStepThreads / S - 1) / (kStepThreads / S);
   // a few groups of channels a block share its row's B and C, while that leaves eight blocks for every SM
   int per = 1;
   while (per < 4 && (long long)p.T * ((groups + 2 * per - 1) / (2 * per)) >= 8 * 148) per *= 2;
   if (p.T > 65535) return (int)cudaErrorInvalidValue;
-  return launch(ssm_step_kernel<S, PCS, XT>, dim3((unsigned)((groups + per - 1) / per), (unsigned)p.T), dim3(kSsmThreads), 0, stream, 1, p, per);
+  return launch(ssm_step_kernel<S, PCS, XT>, dim3((unsigned)((groups + per - 1) / per), (unsigned)p.T), dim3(kStepThreads), 0, stream, 1, p, per);
 }
 template <int S, int PCS>
 static int launch_step(const MmbSsmParams& p, cudaStream_t stream) {
@@ -646,13 +708,14 @@ MMB_API int mmb_ssm_scan(const MmbSsmParams* pp, cudaStream_t stream) {
   const MmbSsmParams& p = *pp;
   if (p.T <= 0 || p.D <= 0) return 0;
   if (p.S < 0 || p.N < 1 || p.N > 128 || p.cu_seqlens == nullptr) return (int)cudaErrorInvalidValue;
-  // Lanes a channel: few while there are blocks for every SM, more when a warp would be alone on its scheduler.  Measured (bf16, 16 states; us for
-  // S = 4 / 8 / 16): 4096 tokens of 8192 channels 264 / 350 / 394, 2048 of 2560 92 / 90 / 92, 4096 of 1536 178 / 129 / 133, 2000 of 512 90 / 68 / 54.
+  // Lanes a channel: as many as leave one block to an SM, for a warp alone on its scheduler waits less the fewer states its lanes have; four where
+  // there is more work than that.  Measured (2048 tokens, bf16, 16 states; us for S = 4 / 8 / 16): 768 channels 84 / 67 / 58, 1024 84 / 66 / 58,
+  // 1280 84 / 68 / 70, 2368 84 / 68 / 72, 2560 84 / 94 / 92, 3584 85 / 95 / 120; 4096 tokens of 8192 244 / 326 / 390.
   const long long width = (long long)p.D * (p.S > 0 ? p.S : 1);
-  if (p.N <= 8) return width >= 4096 ? mmb::launch_scan<4, 2, 1, 4>(p, stream) : mmb::launch_scan<8, 1, 1, 4>(p, stream);
+  if (p.N <= 8) return width > 148 * 16 ? mmb::launch_scan<4, 2, 1, 4>(p, stream) : mmb::launch_scan<8, 1, 1, 4>(p, stream);
   if (p.N <= 16) {
-    if (width >= 4096) return mmb::launch_scan<4, 4, 1, 4>(p, stream);
-    return width >= 1024 ? mmb::launch_scan<8, 2, 1, 4>(p, stream) : mmb::launch_scan<16, 1, 1, 2>(p, stream);
+    if (width > 148 * 16) return mmb::launch_scan<4, 4, 1, 4>(p, stream);
+    return width > 148 * 8 ? mmb::launch_scan<8, 2, 1, 4>(p, stream) : mmb::launch_scan<16, 1, 1, 2>(p, stream);
   }
   if (p.N <= 32) return mmb::launch_scan<8, 4, 1, 4>(p, stream);
   // 64 states: two channels a lane halve the shared memory reads of B and C (2000 tokens of 4096 channels, bf16: 199 us against 248 us) once there are

@@ -161,6 +161,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // Pool row of a sequence, or -1 where it is skipped.
 __device__ __forceinline__ long long pool_row(const long long* rows, int s, int pool_rows, int* status) {

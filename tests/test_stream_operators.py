@@ -454,6 +454,18 @@ def test_scan_of_wide_layers(lens, C, N, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lens,C,N,dtype", [([70], 4600, 16, "bf16"), ([131], 4744, 16, "fp16"), ([65], 5919, 13, "fp32"), ([64], 5928, 16, "bf16"), ([130], 7101, 10, "fp32"),
+                                            ([33, 0, 66], 2760, 16, "bf16"), ([129], 7112, 16, "bf16"), ([1, 67], 4140, 16, "fp16"), ([66], 8288, 9, "fp16"),
+                                            ([40], 8280, 16, "fp32"), ([129], 1192, 64, "fp32"), ([70], 1775, 50, "fp32"), ([66], 1400, 64, "bf16"),
+                                            ([70], 1185, 16, "bf16"), ([97], 2368, 16, "fp32")])
+def test_scan_where_wider_blocks_fill_the_sms(lens, C, N, dtype):
+    """Channel counts on both sides of the launcher's choices of five, six and seven scanning warps; tiles of 64 tokens that end inside."""
+    p = ssm_inputs("cuda", lens, C, N, TYPES[dtype], tail=2, seed=C)
+    out, state = run_ssm(p, "cuda")
+    check_ssm(out, state, want_ssm(p))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("B,C,N", [(80, 4100, 16), (300, 2048, 16), (70, 1000, 64), (90, 600, 128)])
 def test_scan_of_a_large_decode_batch(B, C, N):
     p = ssm_inputs("cuda", [B], C, N, torch.bfloat16, seed=4)
