@@ -466,6 +466,16 @@ def test_scan_where_wider_blocks_fill_the_sms(lens, C, N, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C,N,dtype,bc,dt_type", [(8288, 16, "bf16", None, torch.float32), (8280, 12, "fp16", torch.float32, torch.float32), (5928, 16, "bf16", torch.float32, None),
+                                                  (7100, 16, "fp32", torch.bfloat16, None), (4744, 16, "fp32", None, torch.float16), (2400, 16, "bf16", torch.float32, torch.float32),
+                                                  (1300, 64, "fp32", torch.bfloat16, None), (2000, 16, "fp16", torch.float32, None)])
+def test_scan_of_mixed_types_in_every_width(C, N, dtype, bc, dt_type):
+    p = ssm_inputs("cuda", [67], C, N, TYPES[dtype], tail=1, seed=C, bc=bc, dt_type=dt_type)
+    out, state = run_ssm(p, "cuda")
+    check_ssm(out, state, want_ssm(p))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("B,C,N", [(80, 4100, 16), (300, 2048, 16), (70, 1000, 64), (90, 600, 128)])
 def test_scan_of_a_large_decode_batch(B, C, N):
     p = ssm_inputs("cuda", [B], C, N, torch.bfloat16, seed=4)
