@@ -29,6 +29,8 @@
 namespace mmb {
 
 constexpr int kStepThreads = 128;
+constexpr int kSsmSorted = 16;              // up to this many sequences are ordered by length
+constexpr int kSsmSpread = 4;               // up to this many blocks an SM are all resident and spread evenly
 constexpr float kLog2e = 1.4426950408889634f;
 
 // log(1 + e^v) = max(v, 0) + log1p(e), e = e^-|v| in (0, 1]: no overflow, and small steps keep their relative accuracy.  log1p(e) / e is smooth on
@@ -205,8 +207,24 @@ __global__ void __launch_bounds__(32 * W + ST) ssm_scan_kernel(const MmbSsmParam
   constexpr int CH = 32 * W / S * R, NP = S * NPL, YS = ssm_y_pitch(CH), kScan = 32 * W, kAll = kScan + ST;
   constexpr int SG = 2 * G > S ? 2 * G : S;                 // tokens between two sums over the lanes: an even number of groups
   extern __shared__ __align__(16) unsigned char sm[];
-  const int seq = blockIdx.x / n_blocks, c0 = (blockIdx.x % n_blocks) * CH;
+  const int c0 = (blockIdx.x % n_blocks) * CH;
+  int seq = blockIdx.x / n_blocks;
   auto start = [&](int s) { return min(max(p.cu_seqlens[s], 0), p.T); };
+  if (p.S > 1 && p.S <= kSsmSorted && seq < p.S && (long long)n_blocks * p.S > 148 * kSsmSpread) {
+    // the longest sequences first, so that none of them begins when the others end (10 sequences of 12 to 1500 tokens, 4096 channels: 165 -> 153 us;
+    // shortest first 189).  Every block sorts for itself, about 1 us: not worth it for many short sequences (100 of them 94 -> 121 us).
+    int* len = reinterpret_cast<int*>(sm);
+    for (int i = threadIdx.x; i < p.S; i += kAll) len[i] = max(0, start(i + 1) - start(i));
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.S; i += kAll) {
+      int rank = 0;
+      for (int j = 0; j < p.S; ++j) rank += len[j] > len[i] || (len[j] == len[i] && j < i);
+      if (rank == seq) len[p.S] = i;
+    }
+    __syncthreads();
+    seq = len[p.S];
+    __syncthreads();
+  }
   const int begin = start(seq), end = seq < p.S ? max(begin, start(seq + 1)) : p.T;
   if (begin >= end) return;
   long long row = -1;
@@ -642,7 +660,7 @@ static int launch_scan_t(const MmbSsmParams& p, cudaStream_t stream) {
   // a grid of a few blocks a SM is not spread evenly by itself: ask for so much shared memory that no SM takes more than its share
   constexpr int kSmem = 227 * 1024;
   const long long share = ((long long)nb * p.S + 147) / 148;
-  if (share >= 1 && share <= 4) smem = max(smem, (size_t)(kSmem / share - 1024) / 128 * 128);
+  if (share >= 1 && share <= kSsmSpread) smem = max(smem, (size_t)(kSmem / share - 1024) / 128 * 128);
   static std::atomic<unsigned long long> done{0};
   const int e = allow_smem(ssm_scan_kernel<S, NPL, R, G, W, ST, TT, XT>, kSmem, done);
   if (e) return e;

@@ -466,6 +466,15 @@ def test_scan_where_wider_blocks_fill_the_sms(lens, C, N, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[3, 0, 40, 40, 1, 33, 0, 66], [5] * 16, [20, 1] * 8, [7] * 17])
+def test_scan_of_sequences_in_order_of_length(lens):
+    """Equal and empty ones among them; one more than are ordered."""
+    p = ssm_inputs("cuda", lens, 2560, 16, torch.bfloat16, tail=3, seed=len(lens))
+    out, state = run_ssm(p, "cuda")
+    check_ssm(out, state, want_ssm(p))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("C,N,dtype,bc,dt_type", [(8288, 16, "bf16", None, torch.float32), (8280, 12, "fp16", torch.float32, torch.float32), (5928, 16, "bf16", torch.float32, None),
                                                   (7100, 16, "fp32", torch.bfloat16, None), (4744, 16, "fp32", None, torch.float16), (2400, 16, "bf16", torch.float32, torch.float32),
                                                   (1300, 64, "fp32", torch.bfloat16, None), (2000, 16, "fp16", torch.float32, None)])
