@@ -226,9 +226,33 @@ void sink_decode(const Tensor& q, const Tensor& k, const Tensor& v, const OptT& 
   check(mmb_sink_decode(&p, cur_stream()), "sink_decode");
 }
 
+// The same with an output that is made here: one call from Python instead of two.
+Tensor causal_conv_new(const Tensor& x, const Tensor& w, const OptT& bias, const OptT& state, const OptT& rows, const OptT& fresh,
+                       const OptT& cu_seqlens, int64_t act, c10::optional<at::ScalarType> out_dtype) {
+  Tensor out = at::empty(x.sizes(), x.options().dtype(out_dtype.value_or(x.scalar_type())));
+  causal_conv(x, w, bias, out, state, rows, fresh, cu_seqlens, act, true);
+  return out;
+}
+Tensor ssm_new(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const OptT& D, const OptT& z, const OptT& dt_bias,
+               const OptT& state, const OptT& rows, const OptT& fresh, const OptT& cu_seqlens, bool softplus, c10::optional<at::ScalarType> out_dtype) {
+  Tensor out = at::empty(x.sizes(), x.options().dtype(out_dtype.value_or(x.scalar_type())));
+  ssm(x, dt, A, B, C, D, z, dt_bias, out, state, rows, fresh, cu_seqlens, softplus, true);
+  return out;
+}
+Tensor sink_decode_new(const Tensor& q, const Tensor& k, const Tensor& v, const OptT& k_scale, const OptT& v_scale, const Tensor& block_tables,
+                       const Tensor& ctx_lens, int64_t Hq, int64_t Hkv, int64_t D, int64_t block_size, double scale, int64_t window, int64_t sinks,
+                       int64_t fmt) {
+  Tensor out = at::empty({ctx_lens.numel(), Hq, D}, q.options());
+  sink_decode(q, k, v, k_scale, v_scale, block_tables, ctx_lens, out, Hq, Hkv, D, block_size, scale, window, sinks, fmt, 0);
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(mmb200, m) {
+  m.def("causal_conv_new", &causal_conv_new);
+  m.def("ssm_new", &ssm_new);
+  m.def("sink_decode_new", &sink_decode_new);
   m.def("causal_conv", &causal_conv);
   m.def("ssm", &ssm);
   m.def("sink_decode", &sink_decode);

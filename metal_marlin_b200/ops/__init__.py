@@ -516,12 +516,12 @@ def paged_attention(q, k_pool, v_pool, block_tables, ctx_lens, *, Hq, Hkv, dqk, 
     format and head sizes 64, 128 and 256; one launch splits and joins by itself (``csrc/attention_sinks.cu``), so ``splits`` and
     ``workspace`` do not apply.  A sequence without tokens gives zeros; a block outside the pool hides its tokens and a
     sequence longer than its table ends with it, both reported by :func:`check_status`."""
-    B = ctx_lens.numel()
     if sinks:
         if sinks < 0 or window < 0:
             raise ValueError(f"window and sinks must not be negative, got {window} and {sinks}")
         if window > 0:
             return _sink_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv, block_size, scale, window, sinks, w_uv, out)
+    B = ctx_lens.numel()
     dvo = w_uv.shape[1] if w_uv is not None else dv
     fp8 = isinstance(k_pool, FP8KV)
     if not _use_native(q):
@@ -563,8 +563,8 @@ def _sink_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv,
     quant = isinstance(k_pool, FP8KV)
     if quant and not (isinstance(v_pool, FP8KV) and v_pool.fmt == k_pool.fmt):
         raise ValueError("K and V pools must have one cache format")
-    B = ctx_lens.numel()
     if not _use_native(q):
+        B = ctx_lens.numel()
         if dv not in PREFILL_ATTN_DIMS:
             raise ValueError(f"attention with sinks takes head sizes 64, 128 and 256, got {dv}")
         if Hkv < 1 or Hq % Hkv:
@@ -580,14 +580,12 @@ def _sink_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv,
             return out
         return o
     q = q.contiguous()
-    if out is None:
-        out = torch.empty_like(q) if q.dim() == 3 else torch.empty(B, Hq, dv, dtype=torch.bfloat16, device=q.device)
     _report_on(q.device)
-    if quant:
-        K.mmb200.sink_decode(q, k_pool.data, v_pool.data, k_pool.scale, v_pool.scale, block_tables, ctx_lens, out, Hq, Hkv, dv, block_size,
-                             scale, window, sinks, k_pool.fmt_code, 0)
-    else:
-        K.mmb200.sink_decode(q, k_pool, v_pool, None, None, block_tables, ctx_lens, out, Hq, Hkv, dv, block_size, scale, window, sinks, -1, 0)
+    pools = (k_pool.data, v_pool.data, k_pool.scale, v_pool.scale) if quant else (k_pool, v_pool, None, None)
+    fmt = k_pool.fmt_code if quant else -1
+    if out is None:
+        return K.mmb200.sink_decode_new(q, *pools, block_tables, ctx_lens, Hq, Hkv, dv, block_size, scale, window, sinks, fmt)
+    K.mmb200.sink_decode(q, *pools, block_tables, ctx_lens, out, Hq, Hkv, dv, block_size, scale, window, sinks, fmt, 0)
     return out
 
 
@@ -635,6 +633,9 @@ def causal_conv(x, w, bias=None, *, cu_seqlens, state=None, rows=None, fresh=Non
     from zeros.  A sequence with a negative row is skipped, an empty one leaves its window alone; rows of ``x`` that belong to no
     sequence give zeros (in a caller's ``out``: are left as they were).  Live sequences must have different rows.
     Kernel: ``csrc/causal_conv.cu``; single tokens: :func:`causal_conv_step`."""
+    if out is None and _use_native(x):
+        _report_on(x.device)
+        return K.mmb200.causal_conv_new(x, w, bias, state, rows, fresh, cu_seqlens, act, out_dtype)
     zero = out is None
     out = _stream_out(x, out, out_dtype, x)
     if not _use_native(x):
@@ -648,6 +649,9 @@ def causal_conv_step(x, w, bias=None, *, state, rows=None, act=1, out=None, out_
     """One new token per sequence of :func:`causal_conv`: ``x [B, C]``, row ``i`` continues from ``state[rows[i]]`` (row ``i`` without
     ``rows``) and shifts that window by its input.  A negative row is a padding row: its output is zero (in a caller's ``out``: left
     as it was)."""
+    if out is None and _use_native(x):
+        _report_on(x.device)
+        return K.mmb200.causal_conv_new(x, w, bias, state, rows, None, None, act, out_dtype)
     zero = out is None
     out = _stream_out(x, out, out_dtype, x)
     if not _use_native(x):
@@ -666,6 +670,9 @@ def ssm_scan(x, dt, A, Bm, Cm, *, cu_seqlens, state=None, rows=None, fresh=None,
     projection's output; ``A [Di, N]`` (negative), ``D`` and ``dt_bias [Di]`` fp32, ``N`` 1 to 128.  ``state`` fp32 ``[P, Di, N]`` is a pool of
     states that is read where a sequence starts and written where it ends; ``cu_seqlens``, ``rows``, ``fresh``, skipped and empty
     sequences and rows behind the last one as in :func:`causal_conv`.  Kernel: ``csrc/ssm_scan.cu``; single tokens: :func:`ssm_step`."""
+    if out is None and _use_native(x):
+        _report_on(x.device)
+        return K.mmb200.ssm_new(x, dt, A, Bm, Cm, D, z, dt_bias, state, rows, fresh, cu_seqlens, dt_softplus, out_dtype)
     zero = out is None
     out = _stream_out(x, out, out_dtype, x, dt, z, Bm, Cm)
     if not _use_native(x):
@@ -678,6 +685,9 @@ def ssm_scan(x, dt, A, Bm, Cm, *, cu_seqlens, state=None, rows=None, fresh=None,
 def ssm_step(x, dt, A, Bm, Cm, *, state, rows=None, D=None, z=None, dt_bias=None, dt_softplus=False, out=None, out_dtype=None):
     """One new token per sequence of :func:`ssm_scan`: ``x, dt, z [B, Di]``, ``Bm, Cm [B, N]``; row ``i`` updates ``state[rows[i]]`` in place (row
     ``i`` without ``rows``).  A negative row is a padding row: its output is zero (in a caller's ``out``: left as it was)."""
+    if out is None and _use_native(x):
+        _report_on(x.device)
+        return K.mmb200.ssm_new(x, dt, A, Bm, Cm, D, z, dt_bias, state, rows, None, None, dt_softplus, out_dtype)
     zero = out is None
     out = _stream_out(x, out, out_dtype, x, dt, z, Bm, Cm)
     if not _use_native(x):
