@@ -17,14 +17,16 @@
 //   is transposed inside the warp (movmatrix).
 // With the heads as columns every accumulator belongs to a head; as rows (16 of them) up to 8 heads left half of the accumulators empty and took
 // twice the products for S (fp8, 64 rows: 143 us against 135; 8-bit cache of 256-wide heads 75 against 69).
-// P is split into two 16-bit numbers (P = hi + lo to 2^-16): a single bf16 P would add as much error as rounding the output does.
+// P is split into 16-bit numbers whose sum keeps what its 32 bits hold: three in bf16 (8 bits each), two in f16 (11 each).  A single bf16 P would add as
+// much error as rounding the output does; two leave up to 2^-17 of a probability, visible where values cancel.  The third costs its share of the
+// products: 64 rows 164.6 -> 166.6 us, 16 rows of 256-wide heads 49.7 -> 50.7, 16 query heads a KV head (32 rows, 256 wide) 58.6 -> 63.5.
 //
 // Quantized pools: the codes of every format are exact in f16, so both products run in f16.  Q goes in divided by a power of two per row, undone in
 // the score; the row scale of K multiplies the score and that of V the probability, both in fp32.  Probabilities times value scales are kept in f16's
 // range by a reference for the scales (4 x the largest seen) and a factor of 2^7.
 //
-// Measured (graph replays, heads 32 / 8 of 128, window 4096 + 4, three input sets in turn): 64 rows bf16 166 us = 6.5 TB/s, the measured copy rate;
-// 8 rows 28 us; 1 row 11.8 us.  int8 32 rows 62 us and fp8 64 rows 135 us, 1.5 to 1.6 x the time of their bytes: half the bytes a key, the
+// Measured (graph replays, heads 32 / 8 of 128, window 4096 + 4, three input sets in turn): 64 rows bf16 167 us = 6.5 TB/s, 99 % of the measured
+// copy rate; 8 rows 26.8 us; 1 row 12.0 us.  int8 32 rows 62 us and fp8 64 rows 135 us, 1.5 to 1.6 x the time of their bytes: half the bytes a key, the
 // same instructions a key plus the conversions, so the issue slots bound them (hardware conversions into f16 instead of bf16: int8 117 -> 76 us;
 // 32 keys a tile 76 -> 64; rows padded instead of swizzled changed nothing, 62 -> 63).
 #include <atomic>
@@ -178,6 +180,7 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
   using Cfg = SdCfg<D, F>;
   constexpr int R = WIDE ? 16 : 8, U = Cfg::U, NST = Cfg::NST, NI = D / 32, NJ = D / 64, T = Cfg::T, NT = T / 8, KT = T / 16;
   constexpr bool kScaled = F != kSdBf16;
+  constexpr int kParts = kScaled ? 2 : 3;                        // 16-bit numbers that hold a probability
   extern __shared__ __align__(16) unsigned char sm[];
   __shared__ __align__(16) unsigned char q_sm[R * D * 2];        // 16-byte pieces, placed like the units of K
   __shared__ float ml[kSdWarps][R][2], ml_cta[R][2];
@@ -391,24 +394,26 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
         if constexpr (kScaled) p4[h][k] *= vs[k] * inv;
       }
     }
-    // P as B fragments: [8 keys][8 heads] of this layout, transposed inside the warp
-    uint32_t hi[HT][NT], lw[HT][NT];
+    // P as B fragments: [8 keys][8 heads] of this layout, in kParts numbers whose sum it is, transposed inside the warp
+    uint32_t pf[kParts][HT][NT];
 #pragma unroll
     for (int h = 0; h < HT; ++h)
 #pragma unroll
       for (int k = 0; k < NT; ++k) {
-        const float x = p4[2 * h][k], y = p4[2 * h + 1][k];
-        uint32_t a, b;
-        if constexpr (kScaled) {
-          a = pack16(x, y, 1);
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
-          b = pack16(x - f.x, y - f.y, 1);
-        } else {
-          a = sd_pack(x, y);
-          b = sd_pack(x - __uint_as_float(a << 16), y - __uint_as_float(a & 0xffff0000u));
+        float x = p4[2 * h][k], y = p4[2 * h + 1][k];
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+          uint32_t a;
+          if constexpr (kScaled) {
+            a = pack16(x, y, 1);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+            x -= f.x, y -= f.y;
+          } else {
+            a = sd_pack(x, y);
+            x -= __uint_as_float(a << 16), y -= __uint_as_float(a & 0xffff0000u);
+          }
+          pf[i][h][k] = sd_transpose(a);
         }
-        hi[h][k] = sd_transpose(a);
-        lw[h][k] = sd_transpose(b);
       }
     // O^T += V^T P^T
 #pragma unroll
@@ -427,10 +432,9 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
           const uint32_t a0 = __byte_perm(v[0][m], v[1][m], 0x5410), a1 = __byte_perm(v[0][m], v[1][m], 0x7632);
           const uint32_t a2 = __byte_perm(v[2][m], v[3][m], 0x5410), a3 = __byte_perm(v[2][m], v[3][m], 0x7632);
 #pragma unroll
-          for (int h = 0; h < HT; ++h) {
-            sd_mma<F>(o[jj * 4 + m][h], a0, a1, a2, a3, hi[h][2 * kt], hi[h][2 * kt + 1]);
-            sd_mma<F>(o[jj * 4 + m][h], a0, a1, a2, a3, lw[h][2 * kt], lw[h][2 * kt + 1]);
-          }
+          for (int h = 0; h < HT; ++h)
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) sd_mma<F>(o[jj * 4 + m][h], a0, a1, a2, a3, pf[i][h][2 * kt], pf[i][h][2 * kt + 1]);
         }
       }
     __syncwarp();                                                // the stage may be refilled

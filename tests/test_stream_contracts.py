@@ -1,0 +1,43 @@
+"""What the streaming operators promise beyond their formulas: probabilities of 32 bits, one status word a device, the same answers on the CPU and on the
+GPU for bad pages and uneven batches, and decode steps of whole models that agree with the reference path."""
+import pytest
+import torch
+
+from metal_marlin_b200 import ops
+from test_stream_operators import DEVICES, attention_oracle, half_step
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D,G", [(64, 1), (128, 1), (256, 1), (128, 16)])
+def test_probabilities_keep_32_bits(device, D, G):
+    """Values that cancel: three visible keys of probabilities p0 = 1, p1 and p2 (before the sum), v0 + p1 v1 + p2 v2 = 0 to 2^-16 of v0, so that the output's own
+    rounding is far below that of the probabilities.  One element of q and of every key is not zero, so scores are exact products.
+
+    What 32 bits leave, in units of 2^-24 of w = sum p |v|: exponents x = s log2(e) with |x| <= 2 and two roundings, 2 x 2 x ln 2 < 3; the exponential, two
+    steps of 2^-23, 4; the sum over the keys, four terms aligned to the largest, 2^-23 each, 8.  Together below 16 x 2^-24 = 2^-20.  Probabilities in
+    two bf16 numbers would be up to 2^-17 of p1 off, that is 2^-18 w."""
+    B, Hkv, bs, n, window, sinks = 8, 32, 16, 40, 2, 1
+    g = torch.Generator().manual_seed(D + G)
+    bf = lambda t: t.to(torch.bfloat16).double()
+    slots = B * 48
+    k, v = torch.zeros(slots, Hkv, D, dtype=torch.float64), torch.zeros(slots, Hkv, D, dtype=torch.float64)
+    q = torch.zeros(B, Hkv, G, D, dtype=torch.float64)
+    q[:, :, 1:, 0] = bf(torch.rand(B, Hkv, max(G - 1, 1), generator=g))[:, :, : G - 1]
+    q[:, :, 0, 0] = 1.0
+    first, last = torch.arange(B) * 48, torch.arange(B) * 48 + n - 1
+    k[last - 1, :, 0], k[last, :, 0] = (bf(-0.1 - 1.2 * torch.rand(B, Hkv, generator=g)) for _ in range(2))        # scores 0, s1, s2
+    p1, p2 = k[last - 1, :, :1].exp(), k[last, :, :1].exp()
+    v0 = bf(1 + torch.rand(B, Hkv, D, generator=g))
+    v1 = bf(-v0 / p1)
+    v2 = bf(-(v0 + p1 * v1) / p2)
+    v[first], v[last - 1], v[last] = v0, v1, v2
+    tables = torch.arange(3 * B, dtype=torch.int32).view(B, 3)
+    ctx = torch.full((B,), n, dtype=torch.int32)
+    qb, kb, vb = (t.to(torch.bfloat16).to(device) for t in (q.reshape(B, Hkv * G, D), k, v))
+    got = ops.paged_attention(qb, kb, vb, tables.to(device), ctx.to(device), Hq=Hkv * G, Hkv=Hkv, dqk=D, dv=D, block_size=bs, scale=1.0, window=window, sinks=sinks)
+    got = got.double().cpu().view(B, Hkv, G, D)[:, :, 0]
+    total = 1 + p1 + p2
+    o, w = (v0 + p1 * v1 + p2 * v2) / total, (v0 + p1 * v1.abs() + p2 * v2.abs()) / total
+    assert float((o.abs() / w).max()) < 2.0 ** -15
+    off = (got - o).abs() - half_step(torch.bfloat16) * o.abs()
+    assert (off <= 2.0 ** -20 * w).all(), float((off / w).max() * 2 ** 24)
