@@ -73,14 +73,23 @@ def _use_native(t: torch.Tensor) -> bool:
 _status = {}
 
 
+def _status_key(device) -> torch.device:
+    """One key a device: "cuda" is the current GPU, so that every spelling of a device names the word its kernels report to."""
+    device = torch.device(device)
+    return torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
+
+
 def gemm_status(device) -> torch.Tensor:
-    """Per-device int32[4] status word written by kernels whose bounded waits expire."""
-    key = str(device)
-    if key not in _status:
-        _status[key] = torch.zeros(4, dtype=torch.int32, device=device)
-        if torch.device(device).type == "cuda" and native_available():
-            torch.ops.mmb200.set_status_word(_status[key])     # kernels without a status argument report here too
-    return _status[key]
+    """Per-device int32[4] status word written by kernels whose bounded waits expire or that are given an index outside its pool."""
+    word = _status.get(device)
+    if word is None:
+        key = _status_key(device)
+        word = _status.get(key)
+        if word is None:
+            word = _status[key] = torch.zeros(4, dtype=torch.int32, device=key)
+            if key.type == "cuda" and native_available():
+                torch.ops.mmb200.set_status_word(word)         # kernels without a status argument report here too
+    return word
 
 
 def clear_status(device) -> None:
@@ -88,7 +97,7 @@ def clear_status(device) -> None:
 
 
 def check_status(device) -> int:
-    """Host read of the status word (synchronises).  0 = no wait timed out."""
+    """Host read of the status word (synchronises).  0 = no wait timed out and no index was bad."""
     return int(gemm_status(device)[0].item())
 
 
@@ -595,7 +604,7 @@ _reporting = set()
 def _report_on(device) -> None:
     """Registers the device's status word on first use (kernels report bad block tables and pool rows there)."""
     if device not in _reporting:
-        if str(device) not in _status and torch.cuda.is_current_stream_capturing():
+        if _status_key(device) not in _status and torch.cuda.is_current_stream_capturing():
             return                              # the word would live in the graph's memory; the next call outside a capture registers it
         gemm_status(device)
         _reporting.add(device)

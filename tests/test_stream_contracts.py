@@ -41,3 +41,35 @@ def test_probabilities_keep_32_bits(device, D, G):
     assert float((o.abs() / w).max()) < 2.0 ** -15
     off = (got - o).abs() - half_step(torch.bfloat16) * o.abs()
     assert (off <= 2.0 ** -20 * w).all(), float((off / w).max() * 2 ** 24)
+
+
+def test_one_status_word_a_device(monkeypatch):
+    """"cuda" is the current GPU; its word is that of "cuda:0" there, however it is spelled and whichever is asked for first."""
+    real, made = torch.zeros, []
+
+    def zeros(*shape, device=None, **kw):
+        made.append(str(device))
+        return real(*shape, **kw)
+    monkeypatch.setattr(ops, "_status", {})
+    monkeypatch.setattr(ops, "native_available", lambda: False)
+    monkeypatch.setattr(torch, "zeros", zeros)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    words = [ops.gemm_status(d) for d in ("cuda", "cuda:1", torch.device("cuda"), torch.device("cuda", 1), torch.device("cuda:1"))]
+    assert all(w is words[0] for w in words) and made == ["cuda:1"]
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    assert ops.gemm_status("cuda") is ops.gemm_status("cuda:0") is not words[0]
+    assert ops.gemm_status("cpu") is ops.gemm_status(torch.device("cpu"))
+    assert made == ["cuda:1", "cuda:0", "cpu"]
+
+
+@pytest.mark.gpu
+def test_reports_are_seen_and_cleared_under_every_spelling():
+    """A sequence longer than its table: the code that the kernel leaves on cuda:0, read and cleared through both names in turn."""
+    q, pool = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device="cuda:0"), torch.zeros(32, 1, 64, dtype=torch.bfloat16, device="cuda:0")
+    table, ctx = torch.zeros(1, 2, dtype=torch.int32, device="cuda:0"), torch.tensor([33], dtype=torch.int32, device="cuda:0")
+    for read, other in (("cuda", "cuda:0"), ("cuda:0", "cuda"), (torch.device("cuda"), q.device), (q.device, torch.device("cuda"))):
+        ops.clear_status(read)
+        ops.paged_attention(q, pool, pool, table, ctx, Hq=2, Hkv=1, dqk=64, dv=64, block_size=16, scale=1.0, window=8, sinks=2)
+        assert ops.check_status(read) == ops.check_status(other) == 131
+        ops.clear_status(other)
+        assert ops.check_status(read) == 0
