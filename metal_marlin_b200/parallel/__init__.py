@@ -12,7 +12,7 @@ from typing import List, Optional, Sequence
 
 import torch
 
-from .health import (DeviceWaitExpired, ExpertCapacityOverflow, Heartbeat, PeerFailure, StepGuard, decode_status, make_heartbeat,
+from .health import (BadIndex, DeviceWaitExpired, ExpertCapacityOverflow, Heartbeat, PeerFailure, StepGuard, decode_status, make_heartbeat,
                      raise_for_status)
 from .mesh import DeviceMesh, MeshShape, plan_mesh
 
@@ -190,7 +190,7 @@ def __getattr__(name: str):
 
 
 __all__ = ["Device", "DeviceType", "DeviceMesh", "MeshShape", "plan_mesh", "ParallelMode", "ShardSpec", "shard_tensor", "TensorParallelLinear",
-           "PipelineConfig", "PipelineParallel", "all_reduce", "all_gather", "broadcast", "scatter", "PeerFailure", "DeviceWaitExpired",
+           "PipelineConfig", "PipelineParallel", "all_reduce", "all_gather", "broadcast", "scatter", "PeerFailure", "BadIndex", "DeviceWaitExpired",
            "ExpertCapacityOverflow", "Heartbeat", "StepGuard", "decode_status", "make_heartbeat", "raise_for_status", "TPContext",
            "shard_transformer", "make_context", "even_split", "ExpertParallelMoE", "EPExchange", "shard_transformer_ep", "expert_range",
            "PipelineStage", "pipeline_prefill", "pipeline_decode_step", "stage_layers", "ring_attention", "SymmetricBuffer"]

@@ -33,6 +33,15 @@ class DeviceWaitExpired(RuntimeError):
         self.code, self.what = code, what
 
 
+class BadIndex(RuntimeError):
+    """A kernel was given an index that does not exist: a cache block outside the pool or a sequence longer than its block table (131), a state row outside
+    the pool (130).  Nothing waited and nothing outside the pools was touched: the tokens are hidden, the sequence is skipped."""
+
+    def __init__(self, code: int, what: str):
+        super().__init__(f"bad index given to a kernel (status {code}: {what})")
+        self.code, self.what = code, what
+
+
 class ExpertCapacityOverflow(RuntimeError):
     """The expert-parallel receive buffer was too small for the routed rows (status 120): not a peer failure."""
 
@@ -43,7 +52,7 @@ class ExpertCapacityOverflow(RuntimeError):
 
 def decode_status(code: int):
     """Meaning of a device status word: ``(kind, ranks, text)`` with kind in
-    ``"ok" | "peer" | "local" | "capacity"``.  Only three ranges name a rank: 100-109 tensor-parallel source ``code - 100``,
+    ``"ok" | "peer" | "local" | "capacity" | "index"``.  Only three ranges name a rank: 100-109 tensor-parallel source ``code - 100``,
     121-128 expert-parallel sender ``code - 121``, 140-147 expert-parallel return ``code - 140``."""
     if code == 0:
         return "ok", [], "no wait expired"
@@ -55,6 +64,10 @@ def decode_status(code: int):
         return "peer", [code - 140], f"expert-parallel results from rank {code - 140} did not arrive"
     if code == 120:
         return "capacity", [], "expert-parallel receive buffer overflow"
+    if code == 130:
+        return "index", [], "state row outside its pool, sequence skipped"
+    if code == 131:
+        return "index", [], "cache block outside the pool or sequence longer than its block table, tokens hidden"
     names = {1: "GEMM producer barrier", 2: "GEMM MMA barrier", 3: "GEMM expansion barrier", 4: "GEMM epilogue barrier",
              42: "attention kernel barrier", 110: "GEMM all-gather tile wait", 200: "paged decode row barrier"}
     return "local", [], names.get(code, "unknown wait")
@@ -69,6 +82,8 @@ def raise_for_status(code: int) -> None:
         raise PeerFailure(ranks, f"device-side exchange wait expired (status {code}: {text})")
     if kind == "capacity":
         raise ExpertCapacityOverflow(code)
+    if kind == "index":
+        raise BadIndex(code, text)
     raise DeviceWaitExpired(code, text)
 
 

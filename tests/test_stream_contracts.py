@@ -73,3 +73,31 @@ def test_reports_are_seen_and_cleared_under_every_spelling():
         assert ops.check_status(read) == ops.check_status(other) == 131
         ops.clear_status(other)
         assert ops.check_status(read) == 0
+
+
+def test_bad_indexes_are_no_expired_waits():
+    """Codes 130 and 131 of the status word: an index that does not exist.  No wait ran out and no peer is gone."""
+    from metal_marlin_b200.parallel import BadIndex, DeviceWaitExpired, PeerFailure, decode_status, raise_for_status
+    for code, what in ((130, "row"), (131, "block")):
+        kind, ranks, text = decode_status(code)
+        assert (kind, ranks) == ("index", []) and what in text
+        with pytest.raises(BadIndex) as e:
+            raise_for_status(code)
+        assert e.value.code == code and what in str(e.value) and "wait" not in str(e.value)
+        assert not isinstance(e.value, (DeviceWaitExpired, PeerFailure))
+    assert decode_status(128)[0] == "peer" and decode_status(129)[0] == decode_status(132)[0] == "local" and decode_status(140)[0] == "peer"
+
+
+def test_the_engine_reports_a_bad_index_as_such():
+    """The word that the engine polls after a pass."""
+    from metal_marlin_b200.engine.engine import EngineConfig, LLMEngine
+    from metal_marlin_b200.models.config import get_preset
+    from metal_marlin_b200.models.mmfp4_causal_lm import MMFP4ForCausalLM
+    from metal_marlin_b200.parallel import BadIndex
+    lm = MMFP4ForCausalLM.from_config(get_preset("tiny-llama"), device="cpu", seed=0)
+    eng = LLMEngine(lm.model, EngineConfig(num_kv_blocks=16, block_size=16, max_model_len=64, use_cuda_graphs=False))
+    ops.gemm_status("cpu")[0] = 131
+    with pytest.raises(BadIndex):
+        eng._check_device_status()
+    assert ops.check_status("cpu") == 0
+    eng._check_device_status()
