@@ -172,7 +172,7 @@ def mla_prep(q, kva, w_ukT, kv_norm_w, positions, inv_freq, slots, q_full, cache
 
 def paged_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv, block_size, scale, window=0, sinks=0):
     """Returns bf16 [B, Hq, dv].  ``v_pool`` None means V = K[..., :dv] (MLA latent).  With a window the first ``sinks`` keys
-    stay visible."""
+    stay visible; a block outside the pool then hides its tokens and a sequence longer than its table ends with it (status 131)."""
     B = ctx_lens.numel()
     out = torch.zeros(B, Hq, dv, dtype=torch.float32, device=q.device)
     Gh = Hq // Hkv
@@ -180,13 +180,23 @@ def paged_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv,
     vp = v_pool.view(-1, Hkv, dv) if v_pool is not None else None
     for b in range(B):
         n = int(ctx_lens[b])
-        if n == 0:
+        if sinks and n > block_tables.shape[1] * block_size:
+            n = block_tables.shape[1] * block_size
+            _report(131, q.device)
+        if n <= 0:
             continue
         lo = max(0, n - window) if window > 0 else 0
         tok = torch.arange(lo, n, device=q.device)
         if sinks and lo:
             tok = torch.cat([torch.arange(min(sinks, lo), device=q.device), tok])
         slots = block_tables[b, tok // block_size].long() * block_size + (tok % block_size)
+        if sinks:
+            inside = (slots >= 0) & (slots < kp.shape[0])
+            if not inside.all():
+                _report(131, q.device)
+                slots = slots[inside]
+                if not slots.numel():
+                    continue
         K = kp[slots].to(torch.float32)                                   # [n, Hkv, dqk]
         V = vp[slots].to(torch.float32) if vp is not None else K[..., :dv]
         qb = q[b].view(Hkv, Gh, dqk).to(torch.float32)
@@ -194,6 +204,12 @@ def paged_attention(q, k_pool, v_pool, block_tables, ctx_lens, Hq, Hkv, dqk, dv,
         p = torch.softmax(s, dim=-1)
         out[b] = torch.einsum("hgn,nhd->hgd", p, V).reshape(Hq, dv)
     return out.to(torch.bfloat16)
+
+
+def _report(code: int, device) -> None:
+    """Leaves a code in the device's status word, as the kernels do."""
+    from . import gemm_status
+    gemm_status(device)[0] = code
 
 
 def _need(ok, message: str) -> None:

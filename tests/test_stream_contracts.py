@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from metal_marlin_b200 import ops
-from test_stream_operators import DEVICES, attention_oracle, half_step
+from test_stream_operators import (DEVICES, attention_inputs, attention_oracle, check_attention, half_step, run_attention)
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -101,3 +101,28 @@ def test_the_engine_reports_a_bad_index_as_such():
         eng._check_device_status()
     assert ops.check_status("cpu") == 0
     eng._check_device_status()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("block", [-1, -(2 ** 31), 7, 2 ** 31 - 1])
+def test_blocks_outside_the_pool_hide_their_tokens(device, block):
+    """A page of a sequence that the pool does not have, one step below and above it and at the ends of the type; a sequence with nothing else; one
+    that is longer than its table, and one of negative length.  What is left is the attention of the visible tokens alone, and 131 is reported."""
+    Hq, Hkv, D, bs, window, sinks = 4, 2, 64, 16, 40, 3
+    a = attention_inputs(device, [30, 16, 16, 16], Hq, Hkv, D, bs)                   # seven blocks, five of them in use
+    assert a[1].shape[0] == 7 * bs
+    use = a[3][0, 0], a[3][0, 1], a[3][1, 0], a[3][2, 0]
+    tables = torch.tensor([[use[0], block, use[1]], [block, block, block], [use[2], use[3], use[0]], [use[0], use[1], use[2]]], dtype=torch.int32)
+    ctx = [45, 33, 60, -5]                                                           # the third has places for 48
+    ops.clear_status(device)
+    got = run_attention((*a[:3], tables), ctx, Hq, Hkv, D, bs, window, sinks, device)
+    assert ops.check_status(device) == 131
+    ops.clear_status(device)
+    assert not got[1].any() and not got[3].any()
+    # the same tokens as sequences of their own in a dense cache, every one visible: 2 sinks and the window from 5, without the block 16 .. 31; 0 .. 2 and 8 .. 47
+    for b, pos in ((0, [p for p in range(45) if (p < 3 or p >= 5) and not 16 <= p < 32]), (2, [p for p in range(48) if p < 3 or p >= 8])):
+        slots = torch.tensor([int(tables[b, p // bs]) * bs + p % bs for p in pos])
+        n = len(pos)
+        k, v = (torch.cat([t[slots], torch.zeros(48 - n, Hkv, D, dtype=torch.float64)]) for t in a[4:6])
+        want = attention_oracle(a[0][b: b + 1], k, v, torch.arange(3)[None], [n], Hkv, bs, D ** -0.5, n, 1)
+        check_attention(got[b: b + 1], want)
