@@ -259,6 +259,8 @@ def _sequences(x, state, c, n, rows, fresh, cu):
     for i in range(S):
         b = min(max(at[i], 0), x.shape[0])
         length = min(max(at[i + 1], b), x.shape[0]) - b
+        if length > 0 and state is not None and own[i] >= state.shape[0]:
+            _report(130, x.device)
         if length > 0 and (state is None or 0 <= own[i] < state.shape[0]):
             out.append((b, length, None if state is None else own[i], bool(new[i])))
     return out

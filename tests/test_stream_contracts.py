@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from metal_marlin_b200 import ops
-from test_stream_operators import (DEVICES, attention_inputs, attention_oracle, check_attention, half_step, run_attention)
+from test_stream_operators import (DEVICES, attention_inputs, attention_oracle, check_attention, check_conv, check_ssm, conv_inputs, conv_oracle, half_step, run_attention,
+                                   run_ssm, spans, ssm_inputs, want_ssm)
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -126,3 +127,26 @@ def test_blocks_outside_the_pool_hide_their_tokens(device, block):
         k, v = (torch.cat([t[slots], torch.zeros(48 - n, Hkv, D, dtype=torch.float64)]) for t in a[4:6])
         want = attention_oracle(a[0][b: b + 1], k, v, torch.arange(3)[None], [n], Hkv, bs, D ** -0.5, n, 1)
         check_attention(got[b: b + 1], want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_rows_outside_the_pool_are_skipped_and_reported(device):
+    """Prompts and single tokens: a row behind the pool is reported, a negative one is padding, an empty sequence is neither."""
+    x, w, b, state, rows, fresh, cu = conv_inputs(device, [3, 0, 4, 5], 8, 4, torch.bfloat16)
+    for bad, code in (([1, 99, -1, 2], 0), ([1, 2, 7, -1], 130), ([1, 2, 3, 2 ** 62], 130)):
+        pool, rows = state.clone(), torch.tensor(bad)
+        ops.clear_status(device)
+        out = ops.causal_conv(x, w, b, cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=device), state=pool, rows=rows.to(device), fresh=fresh.to(device))
+        assert ops.check_status(device) == code
+        check_conv(out, pool, *conv_oracle(x, w, b, state, spans(cu, fresh, bad), 1))
+    p = ssm_inputs(device, [5, 6], 8, 16, torch.bfloat16)
+    p["rows"] = torch.tensor([1, 99])
+    ops.clear_status(device)
+    out, pool = run_ssm(p, device)
+    assert ops.check_status(device) == 130
+    check_ssm(out, pool, want_ssm(p))
+    for rows, code in (([0, -1], 0), ([4, 1], 130)):
+        ops.clear_status(device)
+        ops.ssm_step(p["x"][:2], p["dt"][:2], p["A"], p["Bm"][:2], p["Cm"][:2], state=p["state"].clone(), rows=torch.tensor(rows, device=device))
+        assert ops.check_status(device) == code
+    ops.clear_status(device)
