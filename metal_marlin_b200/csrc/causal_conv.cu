@@ -8,9 +8,9 @@
 // activated and stored as a whole, with one choice by type for each.  An input is read (TT + K - 1) / TT times, the repeats from L2.  Tiles are cut
 // per sequence, not over the flat token axis: with TT >= K - 1 only a sequence's first tile reads its old window, and the same thread writes the
 // new one (from x, or from the old window where the sequence is shorter than it), so the window is updated in place without a second launch.
-// Tile i belongs to the sequence s with base(s) <= i < base(s + 1), base(s) = cu[s] / TT + s: at least ceil(len / TT) tiles a sequence, found by
-// bisection, nothing counted on the host.  Measured, 8111 rows of 10240 channels, 4 taps, bf16: 71 us = 4.7 TB/s (the bytes 51 us, two special
-// functions a value 37).  Without the activation it takes 66 us, with 24 instead of 16 warps an SM or 16-byte instead of 8-byte loads the same: bound by
+// Tile i belongs to the sequence s with base(s) <= i < base(s + 1), base(s) = cu[s] / TT + s + 1: at least ceil(len / TT) tiles a sequence, found by
+// bisection, nothing counted on the host; the rows in front of the first sequence and behind the last one are sequences -1 and S.
+// Measured, 8111 rows of 10240 channels, 4 taps, bf16: 71 us = 4.7 TB/s (the bytes 51 us, two special functions a value 37).  Without the activation it takes 66 us, with 24 instead of 16 warps an SM or 16-byte instead of 8-byte loads the same: bound by
 // the waves' starts and by reading and writing at once, not by arithmetic.  What it took: conversions between the loads of a batch 332 us; a choice by
 // type at every value 93; arithmetic on one value instead of two an instruction 75.
 //
@@ -153,15 +153,15 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCaus
   __syncthreads();
   if (tile >= n_tiles) return;
   auto start = [&](int s) { return near ? starts[s] : min(max(p.cu_seqlens[s], 0), p.T); };
-  // last sequence whose first tile is at or before this one; number S is the rows behind the last sequence
-  int lo = 0, hi = p.S;
+  // last sequence whose first tile is at or before this one; number -1 is the rows in front of the first sequence, number S those behind the last
+  int lo = -1, hi = p.S;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (start(mid) / TT + mid <= tile) lo = mid;
+    if (start(mid) / TT + mid + 1 <= tile) lo = mid;
     else hi = mid - 1;
   }
-  const int s = lo, begin = start(s), end = s < p.S ? max(begin, start(s + 1)) : p.T;
-  const long long first = (tile - (begin / TT + s)) * TT;
+  const int s = lo, begin = s < 0 ? 0 : start(s), end = s < p.S ? max(begin, start(s + 1)) : p.T;
+  const long long first = (tile - (begin / TT + s + 1)) * TT;
   if (first < 0 || first >= end - begin) return;
   const int t0 = begin + (int)first, t1 = min(end, t0 + TT);
   Raw<V, ES> xr[U], wr[W];
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kConvThreads) causal_conv_kernel(const MmbCaus
       ld_raw<V, ES>(p.x, (long long)(t0 - W + j) * p.ldx + c0, wr[j]);
   }
   long long row = -1;
-  bool live = s < p.S;
+  bool live = s >= 0 && s < p.S;
   if (live && p.state) {
     row = pool_row(p.rows, s, p.pool_rows, p.status);
     live = row >= 0;

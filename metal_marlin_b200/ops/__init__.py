@@ -636,11 +636,11 @@ def causal_conv(x, w, bias=None, *, cu_seqlens, state=None, rows=None, fresh=Non
     ``y[t, c] = silu(bias[c] + sum_k w[c, k] x[t - K + 1 + k, c])`` (``act=0``: no SiLU).
 
     ``x [T, C]`` (bf16, fp16 or fp32, any row stride), ``w [C, K]`` with ``K`` 2 to 8, ``bias [C]`` of ``w``'s type.  Sequence ``i`` is the rows
-    ``cu_seqlens[i] .. cu_seqlens[i + 1]`` (int32 ``[S + 1]`` on the device, starting at 0).  ``state`` fp32 ``[P, C, K - 1]`` is a pool of
+    ``cu_seqlens[i] .. cu_seqlens[i + 1]`` (int32 ``[S + 1]`` on the device, not decreasing).  ``state`` fp32 ``[P, C, K - 1]`` is a pool of
     windows, the last inputs of each sequence with the oldest first: sequence ``i`` continues from row ``rows[i]`` (int64; row ``i``
     without ``rows``), or from zeros where ``fresh[i]`` is set, and leaves its new window there.  Without a pool every sequence starts
     from zeros.  A sequence with a negative row is skipped, an empty one leaves its window alone; rows of ``x`` that belong to no
-    sequence give zeros (in a caller's ``out``: are left as they were).  Live sequences must have different rows.
+    sequence, in front of the first or behind the last, give zeros (in a caller's ``out``: are left as they were).  Live sequences must have different rows.
     Kernel: ``csrc/causal_conv.cu``; single tokens: :func:`causal_conv_step`."""
     if out is None and _use_native(x):
         _report_on(x.device)

@@ -150,3 +150,33 @@ def test_rows_outside_the_pool_are_skipped_and_reported(device):
         ops.ssm_step(p["x"][:2], p["dt"][:2], p["A"], p["Bm"][:2], p["Cm"][:2], state=p["state"].clone(), rows=torch.tensor(rows, device=device))
         assert ops.check_status(device) == code
     ops.clear_status(device)
+
+
+def poisoned(device, *shape, dtype):
+    """Leaves NaN where the next tensor of this size is likely to be made."""
+    torch.full(shape, float("nan"), dtype=dtype, device=device)
+
+
+# rows in front of the first sequence, lengths, rows behind the last
+FRONTS = [(1, [5], 0), (3, [0, 9], 2), (8, [20], 5), (70, [3, 0, 130], 0), (131, [], 9), (7, [0, 0], 3), (64, [1] * 20, 1), (9, [], 0)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("front,lens,tail", FRONTS)
+@pytest.mark.parametrize("C,dtype", [(8, "bf16"), (7, "fp32"), (2048, "fp16")])
+def test_conv_with_rows_in_front_of_the_first_sequence(device, front, lens, tail, C, dtype):
+    """They belong to no sequence: zeros in a new output, left alone in the caller's, and no part of any window."""
+    t = {"bf16": torch.bfloat16, "fp32": torch.float32, "fp16": torch.float16}[dtype]
+    x, w, b, state, rows, fresh, cu = conv_inputs(device, [front] + lens, C, 4, t, tail=tail)
+    cu, rows, fresh = cu[1:], rows[1:], fresh[1:]
+    x[:front] = float("nan")
+    want = conv_oracle(torch.nan_to_num(x), w, b, state, spans(cu, fresh, rows.tolist()), 1)
+    call = dict(cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=device), rows=rows.to(device), fresh=fresh.to(device))
+    pool = state.clone()
+    poisoned(device, *x.shape, dtype=t)
+    out = ops.causal_conv(x, w, b, state=pool, **call)
+    assert not out[:front].any() and not out[cu[-1]:].any()
+    check_conv(out, pool, *want)
+    pool, into = state.clone(), torch.full_like(x, 7.0)
+    assert ops.causal_conv(x, w, b, state=pool, out=into, **call) is into
+    assert (into[:front] == 7).all() and (into[cu[-1]:] == 7).all() and torch.equal(into[front: cu[-1]], out[front: cu[-1]])
