@@ -226,7 +226,8 @@ __global__ void __launch_bounds__(32 * W + ST) ssm_scan_kernel(const MmbSsmParam
     __syncthreads();
   }
   const int begin = start(seq), end = seq < p.S ? max(begin, start(seq + 1)) : p.T;
-  if (begin >= end) return;
+  const int front = seq < p.S ? 0 : start(0);     // the last block also has the rows in front of the first sequence
+  if (begin >= end && front == 0) return;
   long long row = -1;
   bool live = seq < p.S;
   if (live && p.state) {
@@ -235,9 +236,10 @@ __global__ void __launch_bounds__(32 * W + ST) ssm_scan_kernel(const MmbSsmParam
   }
   if (!live) {                                    // rows of no live sequence
     if (p.zero_dead)
-      for (long long i = threadIdx.x; i < (long long)(end - begin) * CH; i += kAll) {
+      for (long long i = threadIdx.x; i < ((long long)(end - begin) + front) * CH; i += kAll) {
         const int c = c0 + (int)(i % CH);
-        if (c < p.D) st1(p.out, (begin + i / CH) * p.ldo + c, ot, 0.f);
+        const long long t = i / CH;
+        if (c < p.D) st1(p.out, (t < front ? t : t - front + begin) * p.ldo + c, ot, 0.f);
       }
     return;
   }

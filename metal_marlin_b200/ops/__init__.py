@@ -678,7 +678,7 @@ def ssm_scan(x, dt, A, Bm, Cm, *, cu_seqlens, state=None, rows=None, fresh=None,
     ``x, dt, z [T, Di]`` and ``Bm, Cm [T, N]`` are bf16, fp16 or fp32 (``Bm`` and ``Cm`` alike) with any row stride, so they can be slices of a
     projection's output; ``A [Di, N]`` (negative), ``D`` and ``dt_bias [Di]`` fp32, ``N`` 1 to 128.  ``state`` fp32 ``[P, Di, N]`` is a pool of
     states that is read where a sequence starts and written where it ends; ``cu_seqlens``, ``rows``, ``fresh``, skipped and empty
-    sequences and rows behind the last one as in :func:`causal_conv`.  Kernel: ``csrc/ssm_scan.cu``; single tokens: :func:`ssm_step`."""
+    sequences and rows of no sequence as in :func:`causal_conv`.  Kernel: ``csrc/ssm_scan.cu``; single tokens: :func:`ssm_step`."""
     if out is None and _use_native(x):
         _report_on(x.device)
         return K.mmb200.ssm_new(x, dt, A, Bm, Cm, D, z, dt_bias, state, rows, fresh, cu_seqlens, dt_softplus, out_dtype)

@@ -180,3 +180,22 @@ def test_conv_with_rows_in_front_of_the_first_sequence(device, front, lens, tail
     pool, into = state.clone(), torch.full_like(x, 7.0)
     assert ops.causal_conv(x, w, b, state=pool, out=into, **call) is into
     assert (into[:front] == 7).all() and (into[cu[-1]:] == 7).all() and torch.equal(into[front: cu[-1]], out[front: cu[-1]])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("front,lens,tail", FRONTS)
+@pytest.mark.parametrize("C,N", [(8, 16), (7, 5), (300, 64)])
+def test_scan_with_rows_in_front_of_the_first_sequence(device, front, lens, tail, C, N):
+    """The same of the selective scan."""
+    p = ssm_inputs(device, [front] + lens, C, N, torch.bfloat16, tail=tail)
+    p["cu"], p["rows"], p["fresh"] = p["cu"][1:], p["rows"][1:], p["fresh"][1:]
+    want = want_ssm(p)
+    for name in ("x", "z", "dt", "Bm", "Cm"):
+        p[name][:front] = float("nan")
+    poisoned(device, *p["x"].shape, dtype=torch.bfloat16)
+    out, state = run_ssm(p, device)
+    assert not out[:front].any() and not out[p["cu"][-1]:].any()
+    check_ssm(out, state, want)
+    into = torch.full((p["x"].shape[0], C), 7.0, dtype=torch.bfloat16, device=device)
+    run_ssm(p, device, out=into)
+    assert (into[:front] == 7).all() and (into[p["cu"][-1]:] == 7).all() and torch.equal(into[front: p["cu"][-1]], out[front: p["cu"][-1]])
