@@ -679,10 +679,18 @@ static int launch_scan_w(const MmbSsmParams& p, cudaStream_t stream) {
          : p.xt == 1 ? launch_scan_t<S, NPL, R, G, W, ST, TT, 1>(p, stream)
                      : launch_scan_t<S, NPL, R, G, W, ST, TT, 2>(p, stream);
 }
+// The same where x is fp32.
+template <int S, int NPL, int R, int G, int W, int ST, int TT>
+static int launch_scan_f(const MmbSsmParams& p, cudaStream_t stream) {
+  const bool same = p.dtt == 2 && p.bt == 2 && p.ot == 2 && (p.z == nullptr || p.zt == 2);
+  return same ? launch_scan_t<S, NPL, R, G, W, ST, TT, 2>(p, stream) : launch_scan_t<S, NPL, R, G, W, ST, TT, 3>(p, stream);
+}
 // Blocks of four scanning warps, unless some SMs would get two of them where wider blocks give every SM at most one: then the SM with the most
 // work has W warps instead of eight.  A block that has its SM to itself needs more staging warps, or they are what the scan waits for, and the wide
 // ones longer tiles, as there is no other block to run while the two roles hand over.  Measured (bf16, 16 states; us for four and for W warps):
-// 4096 tokens of 8192 channels 263 / 244 (7), 2048 of 7000 136 / 117 (6), 2048 of 5120 134 / 112 (5); 64 states, 1531 of 1536, fp32 95 / 82 (6).  One
+// 4096 tokens of 8192 channels 263 / 244 (7), 2048 of 7000 136 / 117 (6), 2048 of 5120 134 / 112 (5).  33 to 64 states: six warps where x is fp32, at
+// 1192 / 1400 / 1776 channels (1531 tokens, us for four and for six warps) 92 / 80, 92 / 81, 92 / 81, with bf16 B and C 104 / 90; with a 16-bit x a tile of six
+// warps is 12 channels or 24 bytes wide, no whole 16-byte pieces: bf16 94 / 93 there and 27.7 / 29.3 for 400 tokens, so four.  One
 // block of four warps an SM, with four and with eight staging warps: 2048 of 4096 94 / 84, 4096 of 1536 (eight lanes a channel) 134 / 129.
 // fp32 inputs with a 16-bit gate and output: 2048 of 5120 160 / 138, 2048 of 4096 140 / 105.
 template <int S, int NPL, int R, int G>
@@ -700,7 +708,7 @@ static int launch_scan(const MmbSsmParams& p, cudaStream_t stream) {
     if (one_each(4)) return launch_scan_w<S, NPL, R, G, 4, 256, 32>(p, stream);
   }
   if constexpr (S == 16 && NPL == 4 && R == 1) {
-    if (!one_each(4) && one_each(6)) return launch_scan_w<S, NPL, R, G, 6, 384, 64>(p, stream);
+    if (p.xt == 2 && !one_each(4) && one_each(6)) return launch_scan_f<S, NPL, R, G, 6, 384, 64>(p, stream);
   }
   return launch_scan_w<S, NPL, R, G, 4, 128, 32>(p, stream);
 }
