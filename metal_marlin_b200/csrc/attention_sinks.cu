@@ -72,16 +72,6 @@ __device__ __forceinline__ int sd_unit_v(int r, int u) {
   return u;
 }
 
-__device__ __forceinline__ float sd_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t sd_pack(float a, float b) {
-  const bf162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // 8 cached codes at `p` as four f16 pairs (all formats are exact in it).  int8: 0x6400 + u is the f16 number 1024 + u for 0 <= u < 256.
 template <int F>
 __device__ __forceinline__ void sd_load8_f16(const unsigned char* p, uint32_t (&w)[4]) {
@@ -148,16 +138,9 @@ __device__ __forceinline__ void sd_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
   else mma_f16_16816(d, a0, a1, a2, a3, b0, b1);
 }
 
-__device__ __forceinline__ void sd_cp16(void* dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void sd_cp4(void* dst, const void* src, bool ok) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ void sd_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void sd_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 __device__ __forceinline__ uint32_t sd_remote(uint32_t addr, int rank) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
@@ -250,8 +233,8 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
         const int e = i * 32 + lane, r = e / U, u = e % U;
         const int sl = __shfl_sync(0xffffffffu, slot, r);
         const long long at = (long long)max(sl, 0) * row_stride + (head_at + u * 16);
-        sd_cp16(st + (r * U + sd_unit_k<U, Cfg::piece>(r, u)) * 16, reinterpret_cast<const unsigned char*>(p.k) + at, sl >= 0);
-        sd_cp16(st + Cfg::tile_bytes / 2 + (r * U + sd_unit_v<U, Cfg::piece>(r, u)) * 16, reinterpret_cast<const unsigned char*>(p.v) + at, sl >= 0);
+        cp_async16(st + (r * U + sd_unit_k<U, Cfg::piece>(r, u)) * 16, reinterpret_cast<const unsigned char*>(p.k) + at, sl >= 0);
+        cp_async16(st + Cfg::tile_bytes / 2 + (r * U + sd_unit_v<U, Cfg::piece>(r, u)) * 16, reinterpret_cast<const unsigned char*>(p.v) + at, sl >= 0);
       }
       if constexpr (kScaled) {
         const long long at = slot >= 0 ? (long long)slot * p.Hkv + hk : 0;
@@ -263,7 +246,7 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
         }
       }
     }
-    sd_commit();
+    cp_async_commit();
   };
 
   constexpr int HT = R / 8;                                      // tiles of eight heads
@@ -297,7 +280,7 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
   for (int t = 0; t < mine; ++t) {
     issue(t + NST - 1, next);
     next = slot_of(t + NST);
-    sd_wait<NST - 1>();
+    cp_async_wait<NST - 1>();
     __syncwarp();
     const unsigned char* st = ring + (t % NST) * Cfg::stage_bytes;
     const unsigned char* vt = st + Cfg::tile_bytes / 2;
@@ -370,7 +353,7 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
         const float m = lanes_max(sd_max(p4[h]));
         alpha[h] = beta;
         if (m > mx[h]) {
-          const float f = sd_exp2(mx[h] - m);
+          const float f = exp2_fast(mx[h] - m);
           mx[h] = m;
           l[h] *= f;
           alpha[h] *= f;
@@ -389,7 +372,7 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
       const float ref = mx[h] == -INFINITY ? 0.f : mx[h];
 #pragma unroll
       for (int k = 0; k < NT; ++k) {
-        p4[h][k] = sd_exp2(p4[h][k] - ref);
+        p4[h][k] = exp2_fast(p4[h][k] - ref);
         l[h] += p4[h][k];
         if constexpr (kScaled) p4[h][k] *= vs[k] * inv;
       }
@@ -409,7 +392,7 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
             x -= f.x, y -= f.y;
           } else {
-            a = sd_pack(x, y);
+            a = pack16(x, y, 0);
             x -= __uint_as_float(a << 16), y -= __uint_as_float(a & 0xffff0000u);
           }
           pf[i][h][k] = sd_transpose(a);
@@ -441,7 +424,7 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
   }
 
   // ---- join the warps.  Head r of warp w: maximum and sum in ml, O in the (idle) ring as [w][r][D]
-  sd_wait<0>();
+  cp_async_wait<0>();
   __syncthreads();
 #pragma unroll
   for (int h = 0; h < 2 * HT; ++h) {
@@ -467,7 +450,7 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
       }
   __syncthreads();
   // weights of the warps of row r: 2^(m_w - M)
-  auto weight = [](float mw, float M) { return mw == -INFINITY ? 0.f : sd_exp2(mw - M); };
+  auto weight = [](float mw, float M) { return mw == -INFINITY ? 0.f : exp2_fast(mw - M); };
   if (splits == 1) {
     for (int i = tid; i < heads * D / 4; i += kSdThreads) {
       const int r = i / (D / 4), col = i % (D / 4) * 4;
@@ -483,7 +466,7 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
         a.x = fmaf(f, x.x, a.x), a.y = fmaf(f, x.y, a.y), a.z = fmaf(f, x.z, a.z), a.w = fmaf(f, x.w, a.w);
       }
       const float inv = L == 0.f ? 0.f : 1.f / L;                // a row that sees nothing is zero
-      uint2 w2 = make_uint2(sd_pack(a.x * inv, a.y * inv), sd_pack(a.z * inv, a.w * inv));
+      uint2 w2 = make_uint2(pack16(a.x * inv, a.y * inv, 0), pack16(a.z * inv, a.w * inv, 0));
       *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(p.out) + ((long long)b * p.Hq + head0 + r) * D + col) = w2;
     }
     return;
@@ -521,7 +504,7 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
       a.x = fmaf(f, x.x, a.x), a.y = fmaf(f, x.y, a.y), a.z = fmaf(f, x.z, a.z), a.w = fmaf(f, x.w, a.w);
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    uint2 w2 = make_uint2(sd_pack(a.x * inv, a.y * inv), sd_pack(a.z * inv, a.w * inv));
+    uint2 w2 = make_uint2(pack16(a.x * inv, a.y * inv, 0), pack16(a.z * inv, a.w * inv, 0));
     *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(p.out) + ((long long)b * p.Hq + head0 + r) * D + col) = w2;
   }
   cluster_arrive();                                              // nobody leaves while its shared memory is still read

@@ -49,13 +49,6 @@ __device__ __forceinline__ float softplus(float v) {
   return fmaf(q, e, fmaxf(v, 0.f));
 }
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // softplus of two values; the polynomial takes one instruction a step for both.
 __device__ __forceinline__ void softplus2(float (&v)[2]) {
   const float e0 = exp2_fast(-kLog2e * fabsf(v[0])), e1 = exp2_fast(-kLog2e * fabsf(v[1]));
@@ -150,17 +143,6 @@ template <int V>
 struct Int {
   static constexpr int value = V;
 };
-
-// Pair j of a lane's NPL consecutive values, by 16-byte loads where they are.
-template <int NPL>
-__device__ __forceinline__ f32x2 at2(const float* p, int j) {
-  if constexpr (NPL % 4 == 0) {
-    const ulonglong2 u = reinterpret_cast<const ulonglong2*>(p)[j / 2];
-    return j % 2 ? u.y : u.x;
-  } else {
-    return reinterpret_cast<const f32x2*>(p)[j];
-  }
-}
 
 // Byte offsets of the parts of a block's shared memory.
 struct SsmLayout {
@@ -505,13 +487,8 @@ __global__ void __launch_bounds__(32 * W + ST) ssm_scan_kernel(const MmbSsmParam
   }
 }
 
-// One row's inputs of the single-token kernel as raw bits.  XT: the type of x, dt, z, B and C where they have one type and whole pieces can be
+// Inputs of the single-token kernel as raw bits.  XT: the type of x, dt, z, B and C where they have one type and whole pieces can be
 // loaded, else 3; a choice at run time around every load would keep the loads from being issued together.
-template <int PCS, int XT>
-struct StepRow {
-  float h[PCS][4];
-  uint32_t b[PCS][XT < 2 ? 2 : 4], c[PCS][XT < 2 ? 2 : 4], x, dt, z;
-};
 template <int XT, int W>
 __device__ __forceinline__ void ld_quad(const void* p, long long i, int n, int t, uint32_t (&w)[W]) {
   if constexpr (XT < 2) {

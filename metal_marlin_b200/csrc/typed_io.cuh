@@ -167,6 +167,14 @@ __device__ __forceinline__ float rcp_fast(float x) {
   return y;
 }
 
+// 16 bytes from global to shared memory, zeros where they do not exist.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // Pool row of a sequence, or -1 where it is skipped.
 __device__ __forceinline__ long long pool_row(const long long* rows, int s, int pool_rows, int* status) {
   const long long r = rows ? rows[s] : s;
