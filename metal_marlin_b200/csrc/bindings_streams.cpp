@@ -15,7 +15,7 @@ namespace {
 using torch::Tensor;
 using OptT = c10::optional<Tensor>;
 
-constexpr int64_t kMaxRows = 1 << 30;        // the kernels count rows, sequences and tiles of both in 32 bits
+constexpr int64_t kMaxRows = 1 << 30;        // the kernels count rows, sequences, channels and tiles of them in 32 bits: room for the last tile's end
 constexpr int64_t kMaxGrid = 65535;          // rows of a single-token call
 
 inline cudaStream_t cur_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
@@ -44,11 +44,15 @@ inline const float* opt_f32(const OptT& t, int64_t n, const Tensor& on, const ch
   return t->data_ptr<float>();
 }
 
+inline void check_tokens(const Tensor& x) {
+  TORCH_CHECK_VALUE(x.dim() == 2, "x must be [tokens, channels]");
+  TORCH_CHECK_VALUE(x.size(0) <= kMaxRows && x.size(1) <= kMaxRows, "at most ", kMaxRows, " rows and channels, got ", x.size(0), " and ", x.size(1));
+}
+
 // State pool [rows, c, n], rows / fresh / cu_seqlens of a call over the activation rows of x.
 template <typename P>
 void fill_sequences(P& p, const Tensor& x, const OptT& state, int64_t c, int64_t n, const OptT& rows, const OptT& fresh, const OptT& cu) {
   int64_t S = x.size(0);
-  TORCH_CHECK_VALUE(x.size(0) <= kMaxRows && c <= INT_MAX, "too many rows or channels");
   if (given(cu)) {
     TORCH_CHECK_VALUE(cu->scalar_type() == at::kInt && cu->dim() == 1 && cu->numel() >= 1 && cu->numel() <= kMaxRows && cu->is_contiguous() &&
                           cu->device() == x.device(),
@@ -88,7 +92,7 @@ void fill_sequences(P& p, const Tensor& x, const OptT& state, int64_t c, int64_t
 
 void causal_conv(const Tensor& x, const Tensor& w, const OptT& bias, Tensor out, const OptT& state, const OptT& rows, const OptT& fresh,
                  const OptT& cu_seqlens, int64_t act, bool zero_dead) {
-  TORCH_CHECK_VALUE(x.dim() == 2, "x must be [tokens, channels]");
+  check_tokens(x);
   const int64_t T = x.size(0), C = x.size(1);
   check_2d(x, T, C, x, "x");
   TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) == C && w.size(1) >= 2 && w.size(1) <= 8 && w.is_contiguous(), "w must be contiguous [", C, ", 2 .. 8]");
@@ -122,7 +126,7 @@ void causal_conv(const Tensor& x, const Tensor& w, const OptT& bias, Tensor out,
 
 void ssm(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const OptT& D, const OptT& z, const OptT& dt_bias,
          Tensor out, const OptT& state, const OptT& rows, const OptT& fresh, const OptT& cu_seqlens, bool softplus, bool zero_dead) {
-  TORCH_CHECK_VALUE(x.dim() == 2, "x must be [tokens, channels]");
+  check_tokens(x);
   const int64_t T = x.size(0), Di = x.size(1);
   check_2d(x, T, Di, x, "x");
   check_2d(dt, T, Di, x, "dt");

@@ -231,6 +231,7 @@ def _sequences(x, state, c, n, rows, fresh, cu):
     """Checks of a call over pooled per-sequence state (those of the CUDA binding), then ``(first row, length, pool row or None, starts
     anew)`` of every sequence that is neither empty nor skipped."""
     S = x.shape[0]
+    _need(S <= 1 << 30 and c <= 1 << 30, f"at most 2^30 rows and channels, got {S} and {c}")
     if cu is not None:
         _need(cu.dtype == torch.int32 and cu.dim() == 1 and cu.numel() >= 1 and cu.is_contiguous() and cu.device == x.device,
               "cu_seqlens must be a contiguous int32 vector on the device of x")

@@ -199,3 +199,23 @@ def test_scan_with_rows_in_front_of_the_first_sequence(device, front, lens, tail
     into = torch.full((p["x"].shape[0], C), 7.0, dtype=torch.bfloat16, device=device)
     run_ssm(p, device, out=into)
     assert (into[:front] == 7).all() and (into[p["cu"][-1]:] == 7).all() and torch.equal(into[front: p["cu"][-1]], out[front: p["cu"][-1]])
+
+
+@pytest.mark.parametrize("T,C", [(1, 2 ** 30 + 1), (1, 2 ** 31 - 1), (2 ** 30 + 1, 1)])
+def test_sizes_that_the_kernels_do_not_count_are_refused(T, C):
+    """Rows and channels are numbered in 32 bits, up to the end of the last tile: more than 2^30 of either is refused.  Shapes alone, nothing is allocated."""
+    from metal_marlin_b200 import _build
+    m = lambda *shape, dtype=torch.float32: torch.empty(*shape, device="meta", dtype=dtype)
+    x, w, A, bc, cu = m(T, C, dtype=torch.bfloat16), m(C, 2), m(C, 1), m(T, 1), m(2, dtype=torch.int32)
+    for call in (lambda: ops.causal_conv(x, w, cu_seqlens=cu), lambda: ops.ssm_scan(x, x, A, bc, bc, cu_seqlens=cu)):
+        with pytest.raises(ValueError):
+            call()
+    if T == 1:
+        for call in (lambda: ops.causal_conv_step(x, w, state=m(1, C, 1)), lambda: ops.ssm_step(x, x, A, bc, bc, state=m(1, C, 1))):
+            with pytest.raises(ValueError):
+                call()
+    if _build.load():
+        with pytest.raises(ValueError):
+            torch.ops.mmb200.causal_conv(x, w, None, x, None, None, None, cu, 1, True)
+        with pytest.raises(ValueError):
+            torch.ops.mmb200.ssm(x, x, A, bc, bc, None, None, None, x, None, None, None, cu, False, True)
