@@ -20,15 +20,19 @@
 // P is split into 16-bit numbers whose sum keeps what its 32 bits hold: three in bf16 (8 bits each), two in f16 (11 each).  A single bf16 P would add as
 // much error as rounding the output does; two leave up to 2^-17 of a probability, visible where values cancel.  The third costs its share of the
 // products: 64 rows 164.6 -> 166.6 us, 16 rows of 256-wide heads 49.7 -> 50.7, 16 query heads a KV head (32 rows, 256 wide) 58.6 -> 63.5.
+// The products cut off what they can not add to an accumulator (no rounding), always towards zero: a sum over thousands of keys would drift by 2^-17.  So
+// they sum one tile from zero, and an ordinary addition, rounded to nearest, takes that to O: 64 rows 168.0 -> 169.1 us, fp8 134.8 -> 140.7, fp4 154 -> 156, int4
+// 160 -> 164, 8-bit cache of 256-wide heads 69.3 -> 71.1.  Outputs that are not the nearest bf16 to the exact value (64 rows): 2.0 in 1000 before, 0.23 after; with 32-bit products 0.9.
 //
 // Quantized pools: the codes of every format are exact in f16, so both products run in f16.  Q goes in divided by a power of two per row, undone in
 // the score; the row scale of K multiplies the score and that of V the probability, both in fp32.  Probabilities times value scales are kept in f16's
 // range by a reference for the scales (4 x the largest seen) and a factor of 2^7.
 //
-// Measured (graph replays, heads 32 / 8 of 128, window 4096 + 4, three input sets in turn): 64 rows bf16 167 us = 6.5 TB/s, 99 % of the measured
-// copy rate; 8 rows 26.8 us; 1 row 12.0 us.  int8 32 rows 62 us and fp8 64 rows 135 us, 1.5 to 1.6 x the time of their bytes: half the bytes a key, the
-// same instructions a key plus the conversions, so the issue slots bound them (hardware conversions into f16 instead of bf16: int8 117 -> 76 us;
-// 32 keys a tile 76 -> 64; rows padded instead of swizzled changed nothing, 62 -> 63).
+// Measured (graph replays, heads 32 / 8 of 128, window 4096 + 4, three input sets in turn): 64 rows bf16 169 us = 6.4 TB/s, 97 % of the measured
+// copy rate; 8 rows 27.1 us; 1 row 12.2 us.  64 rows int8 117 us and fp8 141 us, 1.4 and 1.7 x the time of their bytes: half the bytes a key, the
+// same instructions a key plus the conversions, so the issue slots bound them (hardware conversions into f16 instead of bf16: 32 rows of int8 117 -> 76 us;
+// 32 keys a tile 76 -> 64; rows padded instead of swizzled changed nothing, 62 -> 63).  fp4 156 us and int4 164 us for 44 us of bytes: the same
+// bound, with more instructions a conversion.
 #include <atomic>
 #include <cuda_fp4.h>
 
@@ -157,9 +161,14 @@ __device__ __forceinline__ float4 sd_remote_f4(uint32_t addr) {
   return v;
 }
 
+// CTAs an SM that the compiler leaves registers for.  Left alone, 128-wide heads of fp8, fp4 and int4 take 180 to 190 registers, which is two CTAs; held to
+// three they need no spills (9 rows, window 4096, us for two and for three: fp8 39.0 / 36.4, fp4 40.5 / 36.9, int4 42.4 / 38.1; 64 rows 143.6 / 144.5, 162.6 /
+// 156.5, 171.7 / 164).  int8 loses by it (64 rows 121 / 157).
+constexpr int sd_ctas(int D, int F, bool wide) { return !wide && D == 128 && (F == kSdFp8 || F >= kSdFp4) ? 3 : 1; }
+
 // grid (splits, Hkv * head groups, B), clusters of `splits`.  WIDE: 16 query heads a CTA, else 8.
 template <int D, int F, bool WIDE>
-__global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSinkDecodeParams p, int splits, int head_groups, int bs_shift) {
+__global__ void __launch_bounds__(kSdThreads, sd_ctas(D, F, WIDE)) sink_decode_kernel(const MmbSinkDecodeParams p, int splits, int head_groups, int bs_shift) {
   using Cfg = SdCfg<D, F>;
   constexpr int R = WIDE ? 16 : 8, U = Cfg::U, NST = Cfg::NST, NI = D / 32, NJ = D / 64, T = Cfg::T, NT = T / 8, KT = T / 16;
   constexpr bool kScaled = F != kSdBf16;
@@ -398,12 +407,14 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
           pf[i][h][k] = sd_transpose(a);
         }
       }
-    // O^T += V^T P^T
+    // O^T += V^T P^T.  A tile's products are summed from zero, the smallest parts of P first, and added to O once: every product that adds to O itself would
+    // cut O's last bit off
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+    for (int jj = 0; jj < NJ; ++jj) {
+      const int pc = gid + 8 * jj;
+      float d[4][HT][4] = {};
 #pragma unroll
-      for (int jj = 0; jj < NJ; ++jj) {
-        const int pc = gid + 8 * jj;
+      for (int kt = 0; kt < KT; ++kt) {
         uint32_t v[4][4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -417,9 +428,20 @@ __global__ void __launch_bounds__(kSdThreads, 1) sink_decode_kernel(const MmbSin
 #pragma unroll
           for (int h = 0; h < HT; ++h)
 #pragma unroll
-            for (int i = 0; i < kParts; ++i) sd_mma<F>(o[jj * 4 + m][h], a0, a1, a2, a3, pf[i][h][2 * kt], pf[i][h][2 * kt + 1]);
+            for (int i = kParts - 1; i >= 0; --i) sd_mma<F>(d[m][h], a0, a1, a2, a3, pf[i][h][2 * kt], pf[i][h][2 * kt + 1]);
         }
       }
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int h = 0; h < HT; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            float(&x)[4] = o[jj * 4 + m][h];
+            const float2 f = unpack2(add2(pack2(x[e], x[e + 1]), pack2(d[m][h][e], d[m][h][e + 1])));
+            x[e] = f.x, x[e + 1] = f.y;
+          }
+    }
     __syncwarp();                                                // the stage may be refilled
   }
 

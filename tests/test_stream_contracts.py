@@ -219,3 +219,46 @@ def test_sizes_that_the_kernels_do_not_count_are_refused(T, C):
             torch.ops.mmb200.causal_conv(x, w, None, x, None, None, None, cu, 1, True)
         with pytest.raises(ValueError):
             torch.ops.mmb200.ssm(x, x, A, bc, bc, None, None, None, x, None, None, None, cu, False, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "fp8", "int8", "fp4", "int4"])
+@pytest.mark.parametrize("D,G", [(64, 1), (128, 4), (256, 2), (128, 16), (256, 12)])
+def test_long_sums_are_rounded_and_not_cut_off(fmt, D, G):
+    """Enough rows that nobody shares one: each warp keeps one sum over all visible keys, 64 tiles of its own.  Scores repeat from one round of the warps' tiles
+    to the next; values are 256 u in the first round, u with signs in turn in the 62 between, -256 u in the last.  The exact output is zero, while the sum a stays
+    near its largest value.
+
+    Rounded to nearest, a + s and then - s gives a again (it is a multiple of a's step within half a step of a; one step more where a tie was met), whatever
+    the 62 rounds add up to; the first and the last are the same products with other signs.  A tile's own products may lose two steps of theirs, the first and
+    last 256 times as large two of a's each: four steps 2^-23 of at most 257 rounds' worth, against 64 rounds' worth in the denominator, 2.01 x 2^-20 u.
+    Sums that every product cuts off drift by up to a step with each: 2^-15 u."""
+    B, Hkv, bs, rounds, sinks = 320, 1, 16, 64, 16
+    per = 64 if fmt == "bf16" or D == 256 else 128                           # keys of the four warps' tiles
+    m = per * rounds
+    window, n = m - sinks, m + 100
+    g = torch.Generator().manual_seed(D + G)
+    pos = torch.cat([torch.arange(sinks), torch.arange(n - window, n)])
+    k, v = torch.zeros(n + 12, Hkv, D), torch.zeros(n + 12, Hkv, D)
+    k[:, :, 0] = -8.0                                                        # never visible
+    k[pos, 0, 0] = -(torch.rand(per, generator=g) * 2)[torch.arange(m) % per]
+    sign = torch.ones(rounds)
+    sign[2:-1:2], sign[0], sign[-1] = -1.0, 256.0, -256.0
+    u = (1 + torch.rand(D, generator=g)).to(torch.bfloat16).float() if fmt == "bf16" else torch.ones(D)
+    v[pos, 0] = sign[torch.arange(m) // per][:, None] * u
+    assert float(v[pos].double().sum(0).abs().max()) == 0
+    kb, vb = k.to(torch.bfloat16).cuda(), v.to(torch.bfloat16).cuda()
+    if fmt != "bf16":
+        pools = []
+        for t in (kb, vb):
+            pool = ops.FP8KV(n + 12, (Hkv, D), "cuda", fmt)
+            pool.store(torch.arange(n + 12, device="cuda"), t)
+            pools.append(pool)
+        kb, vb = pools
+    q = torch.zeros(B, Hkv * G, D, dtype=torch.bfloat16)
+    q[:, :, 0] = torch.rand(B, Hkv * G, generator=g) + 0.5
+    tables = torch.arange((n + 12) // bs, dtype=torch.int32).expand(B, -1).contiguous().cuda()
+    ctx = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    got = ops.paged_attention(q.cuda(), kb, vb, tables, ctx, Hq=Hkv * G, Hkv=Hkv, dqk=D, dv=D, block_size=bs, scale=1.0, window=window, sinks=sinks)
+    off = got.double().cpu().abs() / u.double()
+    assert float(off.max()) <= 2.02 * 2.0 ** -20, float(off.max()) * 2 ** 20
