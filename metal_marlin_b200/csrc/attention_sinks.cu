@@ -22,7 +22,8 @@
 // products: 64 rows 164.6 -> 166.6 us, 16 rows of 256-wide heads 49.7 -> 50.7, 16 query heads a KV head (32 rows, 256 wide) 58.6 -> 63.5.
 // The products cut off what they can not add to an accumulator (no rounding), always towards zero: a sum over thousands of keys would drift by 2^-17.  So
 // they sum one tile from zero, and an ordinary addition, rounded to nearest, takes that to O: 64 rows 168.0 -> 169.1 us, fp8 134.8 -> 140.7, fp4 154 -> 156, int4
-// 160 -> 164, 8-bit cache of 256-wide heads 69.3 -> 71.1.  Outputs that are not the nearest bf16 to the exact value (64 rows): 2.0 in 1000 before, 0.23 after; with 32-bit products 0.9.
+// 160 -> 164, 8-bit cache of 256-wide heads 69.3 -> 71.1.  Outputs that are not the nearest bf16 to the exact value (64 rows): 2.0 in 1000 before,
+// 0.23 after; with 32-bit products and sums 0.9.
 //
 // Quantized pools: the codes of every format are exact in f16, so both products run in f16.  Q goes in divided by a power of two per row, undone in
 // the score; the row scale of K multiplies the score and that of V the probability, both in fp32.  Probabilities times value scales are kept in f16's

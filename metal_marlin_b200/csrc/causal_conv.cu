@@ -10,12 +10,15 @@
 // new one (from x, or from the old window where the sequence is shorter than it), so the window is updated in place without a second launch.
 // Tile i belongs to the sequence s with base(s) <= i < base(s + 1), base(s) = cu[s] / TT + s + 1: at least ceil(len / TT) tiles a sequence, found by
 // bisection, nothing counted on the host; the rows in front of the first sequence and behind the last one are sequences -1 and S.
-// Measured, 8111 rows of 10240 channels, 4 taps, bf16: 71 us = 4.7 TB/s (the bytes 51 us, two special functions a value 37).  Without the activation it takes 66 us, with 24 instead of 16 warps an SM or 16-byte instead of 8-byte loads the same: bound by
-// the waves' starts and by reading and writing at once, not by arithmetic.  What it took: conversions between the loads of a batch 332 us; a choice by
-// type at every value 93; arithmetic on one value instead of two an instruction 75.
+// Measured, 8111 rows of 10240 channels, 4 taps, bf16: 72 us = 4.6 TB/s (the bytes 51 us, two special functions a value 37), 8 taps 91 us; fp32 109.5 us
+// = 6.1 TB/s (the bytes 102 us).  What is left for 16-bit types is the work of a value, which does not overlap its loads and stores altogether: without
+// the activation 66 us, while fp32 with as many bytes in flight a thread comes near the copy rate; 24 instead of 16 warps an SM or 16-byte instead of 8-byte
+// loads changed nothing.  What it took: conversions between the loads of a batch 332 us; a choice by type at every value 93; arithmetic on one value instead
+// of two an instruction 75.
 //
 // Single tokens.  A thread owns V channels of RB rows: the taps are read once for RB rows, the window (V (K - 1) consecutive floats) moves
-// through registers.  256 rows of 10240 channels: 14.6 us = 5.0 TB/s; 4096 channels of 8 taps, fp32: 16.4 us (windows moved by single floats: 55 us).
+// through registers.  256 rows of 10240 channels: 13.8 us = 4.9 TB/s, fp32 15.5 us = 5.0; 4096 channels of 8 taps, fp32: 17.2 us for 10.3 us of
+// bytes (every lane moves 28 values of its own, so a warp's accesses cover their sectors in several steps; by single floats 55 us).
 #include <atomic>
 
 #include "api_ext.h"

@@ -7,8 +7,10 @@
 // Prompts.  Every step of every state takes one exponential and four fp32 operations; at 16 exponentials a clock and SM the special function
 // unit bounds the scan (16 states, 16-bit activations: 3 x longer than moving the activations through memory), closely followed by the
 // 32 bytes a clock that shared memory returns to each scheduler's registers (8 bytes of B and C a state).  The recurrence itself is one
-// multiply-add deep.  The work is split over channels and over the STATES of a channel, never over time (a second pass over time would
-// double the exponentials): S lanes share a channel, each with NPL states in registers (of R channels where there are lanes to spare).  A block
+// multiply-add deep.  The work is split over channels and over the STATES of a channel, never over time: a second pass over time would
+// double the exponentials, which is too much where they bound the scan.  It is what a narrow layer would need, whose few warps wait for one another's
+// latency and leave that unit idle (2048 tokens of 1024 channels, 16 states: 56 us, the exponentials 7, the bytes 3; 8192 of 64: 210 us).  S lanes
+// share a channel, each with NPL states in registers (of R channels where there are lanes to spare).  A block
 // owns 32 W / S R channels of one sequence and walks it in tiles of 32 or 64 tokens with two roles that meet at named barriers, tile by tile:
 //   * ST / 32 staging warps: the tile's x, dt, z, B, C arrive raw by 16-byte cp.async two tiles ahead; they turn x and dt into (d, d x) pairs, so
 //     softplus is paid once per value and not once per lane, and later add the skip term, apply the gate and store the outputs;
@@ -34,7 +36,8 @@ constexpr int kSsmSpread = 4;               // up to this many blocks an SM are 
 constexpr float kLog2e = 1.4426950408889634f;
 
 // log(1 + e^v) = max(v, 0) + log1p(e), e = e^-|v| in (0, 1]: no overflow, and small steps keep their relative accuracy.  log1p(e) / e is smooth on
-// [0, 1] (its singularity lies at -1), so a polynomial of degree 8 fitted to it is within 2^-24.9; with the roundings of its evaluation 2^-22.4.
+// [0, 1] (its singularity lies at -1), so a polynomial of degree 8 fitted to it is, with its coefficients rounded to fp32, within 2^-23.7 of the value; with the roundings of its
+// evaluation within 2^-22.4.
 __device__ __forceinline__ float softplus(float v) {
   const float e = exp2_fast(-kLog2e * fabsf(v));
   float q = 0.0052326880395412445f;
@@ -520,8 +523,9 @@ __device__ __forceinline__ uint32_t ld_bits(const void* p, long long i, int t) {
 
 // S lanes a channel, each PCS pieces of four states; a block owns `per` neighbouring groups of channels of one row.  What bounds it is the state
 // (read and written once); what keeps it from the memory's rate is the work around it, softplus, gate and sums, which every lane of a channel
-// repeats: two pieces a lane instead of one are worth 78 -> 51 us together with the walk along the row (256 rows of 8192 channels, 16 states: 5.6 TB/s;
-// walking the rows of one group of channels with A in registers instead, 65 us: the accesses of neighbouring blocks lie further apart).
+// repeats: two pieces a lane instead of one together with the walk along the row make it 55 us, 4.8 TB/s (256 rows of 8192 channels, 16 states;
+// walking the rows of one group of channels with A in registers instead, 65 us: the accesses of neighbouring blocks lie further apart).  Inputs of several
+// types take the form XT = 3, which also moves the state and A by single values: bf16 x with fp32 dt, B and C 99 us.
 template <int S, int PCS, int XT>
 __global__ void __launch_bounds__(kStepThreads) ssm_step_kernel(const MmbSsmParams p, int per) {
   const int xt = XT < 3 ? XT : p.xt, dtt = XT < 3 ? XT : p.dtt, zt = XT < 3 ? XT : p.zt, bt = XT < 3 ? XT : p.bt;
